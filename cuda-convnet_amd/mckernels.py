@@ -16,6 +16,7 @@ c_i = ctypes.c_int
 c_f = ctypes.c_float
 c_sz = ctypes.c_size_t
 c_u64 = ctypes.c_ulonglong
+c_ll = ctypes.c_longlong
 
 _CONV_ARGS = [c_i] * 12 + [c_f, c_f, c_fp]          # N, C, imgY, imgX, F, fs, pad, stride, mY, mX, groups, (ps) ...
 
@@ -88,12 +89,19 @@ _SIGS = {
     "mc_compute_logreg_softmax_grad": [c_fp] * 3 + [c_i, c_f, c_i, c_i, c_fp],
     "mc_weights_update": [c_fp] * 3 + [c_sz, c_f, c_f, c_f, c_fp],
     "mc_weights_update_spans": [c_fp] * 4 + [c_i, c_fp],
+    "mc_weights_update_spans_clipped": [c_fp] * 4 + [c_i, c_fp, c_fp],
+    "mc_log_probs": [c_fp, c_i, c_ll, c_ll, c_fp, c_i, c_i, c_i] + [c_fp] * 5 + [c_i, c_fp, c_sz, c_fp],
+    "mc_log_probs_grad": [c_fp, c_i, c_ll, c_ll, c_fp, c_i, c_i, c_i, c_fp, c_fp] + [c_fp, c_f] * 3 + [c_fp, c_ll, c_ll, c_i, c_fp],
+    "mc_grad_spans": [c_fp, c_i, c_fp, c_i, ctypes.POINTER(c_i)],
+    "mc_grad_norm": [c_fp, c_i, c_f, c_fp, c_fp, c_sz, c_fp],
+    "mc_clip_grads": [c_fp, c_i, c_fp, c_fp],
     "mc_describe_conv_filter_acts": [ctypes.c_char_p, c_i, c_i] + [c_i] * 11,
     "mc_device_info": [ctypes.c_char_p, c_i, ctypes.POINTER(c_i)],
 }
 
 NEURONS = {"ident": 0, "relu": 1, "brelu": 2, "abs": 3, "logistic": 4, "tanh": 5, "softrelu": 6,
            "square": 7, "sqrt": 8, "linear": 9}
+F32, F16, BF16, I32 = 0, 1, 2, 3     # element types of the entry points that take one
 POOL_MAX, POOL_AVG = 0, 1
 NEURON_NONE, NEURON_RELU = 0, 1
 
@@ -108,7 +116,8 @@ def exported_symbols():
     """Names every build of the library must export (those include/mc_kernels.h declares)."""
     return sorted(list(_SIGS) + ["mc_last_error", "mc_gemm_workspace_bytes", "mc_conv_weight_grad_workspace_bytes",
                                    "mc_noalloc_scratch_bytes", "mc_conv_split_workspace_bytes", "mc_relu_bits_words",
-                                   "mc_conv_weight_grad_bias_workspace_bytes", "mc_gemm_row_sums_workspace_bytes", "mc_dropout_keep_bytes"])
+                                   "mc_conv_weight_grad_bias_workspace_bytes", "mc_gemm_row_sums_workspace_bytes", "mc_dropout_keep_bytes",
+                                   "mc_log_probs_workspace_bytes", "mc_grad_norm_workspace_bytes"])
 
 
 def lib():
@@ -137,6 +146,10 @@ def lib():
         L.mc_relu_bits_words.restype = c_sz
         L.mc_conv_split_workspace_bytes.argtypes = [c_i] * 9
         L.mc_conv_split_workspace_bytes.restype = c_sz
+        L.mc_log_probs_workspace_bytes.argtypes = [c_i, c_ll, c_ll, c_i, c_i, c_i]
+        L.mc_log_probs_workspace_bytes.restype = c_sz
+        L.mc_grad_norm_workspace_bytes.argtypes = [c_i]
+        L.mc_grad_norm_workspace_bytes.restype = c_sz
         L.mc_dropout_keep_bytes.argtypes = [c_sz]
         L.mc_dropout_keep_bytes.restype = c_sz
         _lib = L
@@ -157,3 +170,24 @@ def device_info():
     n = c_i(0)
     call("mc_device_info", buf, 64, ctypes.byref(n))
     return buf.value.decode(), n.value
+
+
+class GradTensor(ctypes.Structure):
+    """mcGradTensor: one gradient of a list (include/mc_kernels.h)."""
+    _fields_ = [("grad", c_fp), ("out", c_fp), ("count", c_u64), ("scale", c_f), ("gradType", c_i), ("outType", c_i), ("pad", c_i)]
+
+
+class GradSpan(ctypes.Structure):
+    """mcGradSpan, as mc_grad_spans makes them."""
+    _fields_ = [("grad", c_fp), ("out", c_fp), ("count", ctypes.c_uint), ("scale", c_f), ("gradType", c_i), ("outType", c_i)]
+
+
+def grad_spans(tensors):
+    """[(gradient pointer, output pointer or 0, elements, scale, gradient type, output type)] -> the host array of spans, ready to be
+    copied to the device (its bytes are what mc_grad_norm and mc_clip_grads read there)."""
+    list_ = (GradTensor * len(tensors))(*[GradTensor(g, o or None, n, s, gt, ot, 0) for g, o, n, s, gt, ot in tensors])
+    n = c_i(0)
+    call("mc_grad_spans", list_, len(tensors), None, 0, ctypes.byref(n))
+    spans = (GradSpan * n.value)()
+    call("mc_grad_spans", list_, len(tensors), spans, n.value, ctypes.byref(n))
+    return spans

@@ -474,6 +474,77 @@ int mc_compute_softmax_grad(const float* acts, const float* actsGrad, float* tar
 int mc_compute_logreg_softmax_grad(const float* labels, const float* probs, float* target, int add,
                                    float coeff, int numCases, int numOut, mcStream_t stream);
 
+/* ---------------- log probabilities of given classes, entropy, top alternatives ----------------
+ * What mc_softmax + mc_compute_logreg_cost give for a few classes in float32, for any number of classes and three element types,
+ * without the probabilities in memory.  No counterpart in the reference.
+ * logits: element (class j, case n) at j*classStride + n*caseStride (in elements), of `type` MC_F32 / MC_F16 / MC_BF16.  One of the
+ * strides is 1: caseStride == 1 is this library's own (numOut, numCases) matrix (classStride >= numCases), classStride == 1 holds a
+ * case's classes side by side (caseStride >= numOut).  Any element alignment.  labels: numCases class indices, MC_I32, or MC_F32
+ * (whole numbers, at most 2^24 classes); a label outside [0, numOut) means "no class".  With m_n the largest logit of case n:
+ *   maxAndLogSum (2, numCases)   m_n, then ln sum_j exp(x_jn - m_n): their sum is the normaliser ln sum_j exp(x_jn)
+ *   labelLogProbs (numCases)     (x_yn - m_n) - ln sum_j exp(x_jn - m_n); 0 for "no class"
+ *   entropy (numCases)           -sum_j p_jn ln p_jn, in nats; 0 ln 0 = 0
+ *   topClasses, topLogProbs (numTop, numCases)   the numTop <= MC_MAX_TOP classes of the largest logits, largest first, equal logits by
+ *                                class, and their log probabilities; a class whose logit is -inf or NaN is never named: the places
+ *                                that are left hold class -1 and log probability -inf
+ * Each output may be NULL (then it is not computed); topClasses and topLogProbs go together.  Sums are held in float32, whatever
+ * `type` is.  Logits of -inf are classes that are ruled out; a case with nothing else has m = -inf, ln sum = 0, labelLogProbs = -inf
+ * (0 for "no class"), entropy 0.  A case with a NaN or +inf logit gets NaN for its log sum, log probabilities and entropy.
+ * workspace: mc_log_probs_workspace_bytes(...) bytes (0 = none), 16-byte aligned; calls that may overlap in time, captured ones
+ * included, need one each.  Results do not depend on the run: no atomics decide an order.  Outputs must not overlap anything else.
+ * The stream must belong to the current device, as must every pointer. */
+enum { MC_F32 = 0, MC_F16 = 1, MC_BF16 = 2, MC_I32 = 3 };
+#define MC_MAX_TOP 32
+size_t mc_log_probs_workspace_bytes(int type, long long classStride, long long caseStride, int numCases, int numOut, int numTop);
+int mc_log_probs(const void* logits, int type, long long classStride, long long caseStride, const void* labels, int labelType,
+                 int numCases, int numOut, float* labelLogProbs, float* entropy, float* maxAndLogSum, int* topClasses,
+                 float* topLogProbs, int numTop, void* workspace, size_t workspaceBytes, mcStream_t stream);
+/* The gradient with respect to the logits (mc_compute_logreg_softmax_grad generalised).  With p_jn = exp((x_jn - m_n) - logSum_n)
+ * and the per-case weights  a_n = scaleLabel * gradLabel[n] (0 for "no class"),  h_n = scaleEntropy * gradEntropy[n],
+ * z_n = scaleLogZ * gradLogZ[n], a NULL array standing for ones:
+ *   target = (add ? target : 0) + a_n * ([j = y_n] - p_jn) - h_n * p_jn * (ln p_jn + entropy_n) + z_n * p_jn
+ * maxAndLogSum and entropy are what mc_log_probs wrote for these logits; a term whose scale is 0 is left out and its arrays (and
+ * `entropy`) are not read.  target has the logits' type and a layout of the same kind (its own strides; the stride that is 1 is the
+ * same one); it may be the logits themselves with the same strides, else the stretch of
+ * memory it spans must not overlap theirs.  The sum is formed in float32 and rounded to `type` once.
+ * A case whose logits are all -inf has gradient 0.  Top alternatives have no gradient. */
+int mc_log_probs_grad(const void* logits, int type, long long classStride, long long caseStride, const void* labels, int labelType,
+                      int numCases, int numOut, const float* maxAndLogSum, const float* entropy, const float* gradLabel,
+                      float scaleLabel, const float* gradEntropy, float scaleEntropy, const float* gradLogZ, float scaleLogZ,
+                      void* target, long long targetClassStride, long long targetCaseStride, int add, mcStream_t stream);
+
+/* ---------------- global gradient norm and clipping ----------------
+ * No counterpart in the reference.  The gradients of a program are a list of tensors (mcGradTensor, on the host); mc_grad_spans cuts
+ * it into spans once, the caller copies them to the device and hands them to every call, as with mcUpdateSpan.
+ *   mc_grad_norm    norm = sqrt(sum over all elements of (scale_t * grad_ti)^2), in double in a fixed order (bit-identical from run
+ *                   to run); normAndFactor[0] = norm, normAndFactor[1] = min(1, maxNorm / norm), or 0 when the norm is NaN or does not fit float32
+ *   mc_clip_grads   out_ti = (factor * scale_t) * grad_ti, rounded to outType once; zeros when factor is 0 (the step is dropped).
+ *                   Tensors without `out` are passed over
+ * `scale` undoes a loss scale or a learning rate that the gradients carry.  maxNorm > 0; INFINITY measures and never clips. */
+typedef struct {
+    const void* grad;          /* device; any element alignment */
+    void* out;                 /* device: where mc_clip_grads writes (may be grad itself if the types are equal), or NULL */
+    unsigned long long count;  /* elements; 0 is allowed */
+    float scale;
+    int gradType, outType;     /* MC_F32 / MC_F16 / MC_BF16 */
+    int pad;
+} mcGradTensor;
+typedef struct {               /* a stretch of one tensor; made by mc_grad_spans */
+    const void* grad;
+    void* out;
+    unsigned count;
+    float scale;
+    int gradType, outType;
+} mcGradSpan;
+/* Host only: *numSpans = how many spans the list takes; fills `spans` (host, maxSpans of them) unless it is NULL.  Rejects lists whose
+ * outputs overlap one another or a gradient other than their own. */
+int mc_grad_spans(const mcGradTensor* tensors, int numTensors, mcGradSpan* spans, int maxSpans, int* numSpans);
+/* workspace of mc_grad_norm: that many bytes, 16-byte aligned, one per call that may overlap in time */
+size_t mc_grad_norm_workspace_bytes(int numSpans);
+int mc_grad_norm(const mcGradSpan* spansDevice, int numSpans, float maxNorm, float* normAndFactor, void* workspace,
+                 size_t workspaceBytes, mcStream_t stream);
+int mc_clip_grads(const mcGradSpan* spansDevice, int numSpans, const float* normAndFactor, mcStream_t stream);
+
 /* ---------------- SGD update ----------------
  * Weights::update (Kernel/include/layers/weights.cuh:150-164) as one pass:
  *   inc = mom*inc + grad; if (wc > 0) inc -= wc*eps*W; W += inc. */
@@ -494,6 +565,11 @@ typedef struct {
 } mcUpdateSpan;
 int mc_weights_update_spans(float* weights, float* inc, const float* grad, const mcUpdateSpan* spansDevice,
                             int numSpans, mcStream_t stream);
+
+/* mc_weights_update_spans with the clip factor of mc_grad_norm: inc = mom*inc + factor*grad + wceps*W; W += inc (weight decay is not
+ * clipped).  Factor 1 gives mc_weights_update_spans' bits; factor 0 (a norm that is not finite) leaves weights and increments alone. */
+int mc_weights_update_spans_clipped(float* weights, float* inc, const float* grad, const mcUpdateSpan* spansDevice, int numSpans,
+                                    const float* normAndFactor, mcStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -462,3 +462,83 @@ def scatter_channels(gathered, conns, C, N, target=None, scale_targets=0.0, scal
     for k, c in enumerate(conns):
         out[c] = out[c] + g[k]
     return _blend(target, out.reshape(-1, N), scale_targets, scale_output)
+
+
+# --------------------------------------------------------------------------
+# log probabilities, their gradient, gradient norm (no counterpart in the reference)
+# --------------------------------------------------------------------------
+def log_probs(x, labels, top=0):
+    """x (numCases, numOut) in float64.  {max, logSum, logp, entropy, classes, top, meanShift = -sum p (x - max)}, in float64: the
+    log probability of each case's label (0 for labels outside [0, numOut)), the entropy in nats and the `top` classes of the
+    largest logits (equal ones by class; -inf and NaN never named: -1) with their log probabilities, (top, numCases)."""
+    x = np.asarray(x, np.float64)
+    N, V = x.shape
+    y = np.asarray(labels)
+    with np.errstate(invalid="ignore", divide="ignore"):
+        bad = np.isnan(x).any(1) | (x == np.inf).any(1)
+        m = np.where(np.isnan(x), -np.inf, x).max(1)
+        empty = (m == -np.inf) & ~bad
+        shift = np.where(np.isneginf(x), -np.inf, x - np.where(np.isfinite(m), m, 0.0)[:, None])
+        e = np.exp(shift)
+        s = e.sum(1)
+        log_sum = np.where(bad, np.nan, np.where(empty, 0.0, np.log(np.where(empty, 1.0, s))))
+        mean = -np.where(e > 0, e * np.where(e > 0, shift, 0.0), 0.0).sum(1) / np.where(empty, 1.0, s)
+        lp = np.where(empty[:, None], -np.inf, shift - log_sum[:, None])
+        lp[bad] = np.nan
+        ok = (y >= 0) & (y < V)
+        logp = np.where(ok, lp[np.arange(N), np.clip(y, 0, V - 1).astype(np.int64)], 0.0)
+        entropy = np.where(bad, np.nan, np.where(empty, 0.0, log_sum + mean))
+    out = {"max": np.where(bad & (m == -np.inf), np.nan, m), "logSum": log_sum, "logp": logp, "entropy": entropy, "meanShift": np.where(bad, 0.0, mean)}
+    k = min(top, V)
+    order = np.argsort(-np.where(np.isnan(x), -np.inf, x), axis=1, kind="stable")[:, :k]
+    named = np.take_along_axis(np.where(np.isnan(x), -np.inf, x), order, 1) > -np.inf
+    classes, values = np.full((top, N), -1, np.int32), np.full((top, N), -np.inf)
+    classes[:k] = np.where(named, order, -1).T
+    values[:k] = np.where(named, np.take_along_axis(lp, order, 1), -np.inf).T
+    out.update(classes=classes, top=values)
+    return out
+
+
+def _log_probs_terms(x, labels, stats, H, g, h, z):
+    x, stats = np.asarray(x, np.float64), np.asarray(stats, np.float64)
+    N, V = x.shape
+    zero = np.zeros(N)
+    g, h, z = (zero if w is None else np.asarray(w, np.float64) for w in (g, h, z))
+    y = np.asarray(labels)
+    ok = (y >= 0) & (y < V)
+    empty = stats[0] == -np.inf
+    with np.errstate(invalid="ignore"):
+        lp = np.where(np.isneginf(x) & np.isfinite(stats).all(0)[:, None], -np.inf, (x - stats[0][:, None]) - stats[1][:, None])
+        p = np.exp(lp)
+        lp = np.where(p == 0, 0.0, lp)          # p ln p = 0 there
+    hot = np.zeros((N, V))
+    hot[np.arange(N)[ok], y[ok].astype(np.int64)] = 1.0
+    return p, lp, np.where(ok, g, 0.0)[:, None], h[:, None], z[:, None], (zero if H is None else np.asarray(H, np.float64))[:, None], hot, empty
+
+
+def log_probs_grad(x, labels, stats, H, g=None, h=None, z=None):
+    """Gradient with respect to x of sum_n g_n logp_n + h_n entropy_n + z_n (max_n + logSum_n), from stats = (max, logSum) and the
+    entropy H as given: g ([j = y] - p) - h p (ln p + H) + z p; 0 for a case whose logits are all -inf."""
+    p, lp, g, h, z, H, hot, empty = _log_probs_terms(x, labels, stats, H, g, h, z)
+    with np.errstate(invalid="ignore"):
+        d = g * (hot - p) - h * p * (lp + H) + z * p
+    d[empty] = 0.0
+    return d
+
+
+def log_probs_grad_size(x, labels, stats, H, g=None, h=None, z=None):
+    """What a rounding error of log_probs_grad is relative to: its terms without cancellation, times 1 + |ln p| / 8 (p = exp(ln p) has
+    the error of ln p)."""
+    p, lp, g, h, z, H, hot, empty = _log_probs_terms(x, labels, stats, H, g, h, z)
+    with np.errstate(invalid="ignore"):
+        d = np.abs(g) * hot + p * (np.abs(g) + np.abs(h) * (np.abs(lp) + np.abs(H) + 1) + np.abs(z)) * (1 + np.abs(lp) / 8)
+    d[empty] = 0.0
+    return d
+
+
+def grad_norm(grads, scales, max_norm):
+    """(norm, factor) of a list of gradients: sqrt(sum (scale g)^2) and min(1, max_norm / norm), 0 for a norm float32 cannot hold."""
+    norm = float(np.sqrt(sum(float((s * np.asarray(g, np.float64)).ravel() @ (s * np.asarray(g, np.float64)).ravel()) for g, s in zip(grads, scales))))
+    if not np.isfinite(np.float32(norm)):
+        return norm, 0.0
+    return norm, 1.0 if norm <= max_norm else max_norm / norm
