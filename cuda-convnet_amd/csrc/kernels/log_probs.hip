@@ -1,13 +1,18 @@
 // log_probs.hip -- log probabilities of given classes with entropy and top alternatives, and their gradient.
-// With m the largest logit of a case, t_j = x_j - m, s = sum_j e^t_j, w = sum_j t_j e^t_j:
-//   ln p_j = t_j - ln s,   -sum_j p_j ln p_j = ln s - w / s.
+// With m the largest logit of a case, t_j = (x_j - m) log2 e, s = sum_j 2^t_j, w = sum_j t_j 2^t_j:
+//   ln p_j = (x_j - m) - ln s,   -sum_j p_j ln p_j = ln 2 (log2 s - w / s),
+// and (m, s, w) of two sets of classes join into those of their union, so a case may be split over workgroups.
 #include <math.h>
+#include <algorithm>
 #include "mc_types.h"
 
 namespace mc {
 namespace {
 
-constexpr int LT = 256;   // threads of a workgroup
+constexpr int LT = 256;             // threads of a workgroup
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr int kMaxOut = 1 << 30;     // classes: their indices stay within an int wherever a tile ends
+constexpr float kHuge = 1e38f;      // from here on x * log2 e may overflow
 
 struct LogProbArgs {
     const void* logits;
@@ -20,6 +25,15 @@ struct LogProbArgs {
     int numTop;
 };
 
+// What a workgroup leaves of its classes of a case for the joining kernel; its best numTop keys follow in an array of their own.
+struct Part { float m, s, w, pad; };
+struct Parts {
+    Part* stats;                  // (numCases, parts)
+    unsigned long long* keys;     // (numCases, parts, numTop), largest first, 0 = none
+    int parts;
+    int span;                     // classes of a part
+};
+
 // The label of case n, or -1 for "no class".
 __device__ __forceinline__ int label_of(const void* labels, int labelType, int n, int numOut) {
     if (labelType == MC_I32) {
@@ -30,25 +44,55 @@ __device__ __forceinline__ int label_of(const void* labels, int labelType, int n
     return y >= 0.f && y < (float)numOut ? (int)y : -1;
 }
 
-__device__ __forceinline__ float block_max(float v, float* sh) {
-    for (int off = 32; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
-    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
-    __syncthreads();
-    float r = sh[0];
-    for (int i = 1; i < LT / 64; ++i) r = fmaxf(r, sh[i]);
-    __syncthreads();
-    return r;
-}
-__device__ __forceinline__ float block_sum(float v, float* sh) {
-    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
-    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
-    __syncthreads();
-    float r = sh[0];
-    for (int i = 1; i < LT / 64; ++i) r += sh[i];
-    __syncthreads();
-    return r;
-}
+// ---------------------------------------------------------------- groups of threads that share a case
+// A whole workgroup, or one wave of it (whose LDS accesses are in order: there only the compiler has to be held back).
+template <int THREADS>
+struct Group {
+    static_assert(THREADS == LT || THREADS == 64, "");
+    static constexpr int WAVES = THREADS / 64;
+    __device__ static int index() { return THREADS == LT ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / THREADS); }
+    __device__ static int tid() { return threadIdx.x & (THREADS - 1); }
+    __device__ static void sync() {
+        if (THREADS == LT) __syncthreads();
+        else {
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+            __builtin_amdgcn_wave_barrier();
+        }
+    }
+    __device__ static bool any(bool v) { return THREADS == LT ? __syncthreads_or(v) : __any(v); }
+    // sh: WAVES floats of LDS that nobody else uses until the next sync
+    __device__ static float max(float v, float* sh) {
+        for (int off = 32; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
+        if (WAVES == 1) return v;
+        if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+        sync();
+        v = sh[0];
+#pragma unroll
+        for (int i = 1; i < WAVES; ++i) v = fmaxf(v, sh[i]);
+        return v;
+    }
+    __device__ static void sum2(float& a, float& b, float* sh) {
+        for (int off = 32; off > 0; off >>= 1) {
+            a += __shfl_xor(a, off, 64);
+            b += __shfl_xor(b, off, 64);
+        }
+        if (WAVES == 1) return;
+        if ((threadIdx.x & 63) == 0) {
+            sh[threadIdx.x >> 6] = a;
+            sh[WAVES + (threadIdx.x >> 6)] = b;
+        }
+        sync();
+        a = sh[0];
+        b = sh[WAVES];
+#pragma unroll
+        for (int i = 1; i < WAVES; ++i) {
+            a += sh[i];
+            b += sh[WAVES + i];
+        }
+    }
+};
 
+// ---------------------------------------------------------------- top alternatives
 // Orders logits as the top alternatives are ordered: larger logit first, then lower class.  0 = never chosen (-inf, NaN).
 __device__ __forceinline__ unsigned long long top_key(float x, unsigned j) {
     if (!(x > -INFINITY)) return 0;
@@ -62,79 +106,537 @@ __device__ __forceinline__ float key_logit(unsigned long long key) {
 }
 __device__ __forceinline__ int key_class(unsigned long long key) { return (int)(0xffffffffu - (unsigned)key); }
 
-// The k largest keys of a case in one walk over its classes in order: 256 classes at a time against the k-th best so far; what
-// beats it joins the list, which is ordered again by counting, for each key, the larger ones.
-template <class T>
-__device__ void top_by_scan(const T* x, size_t stride, int numOut, int k, unsigned long long* best, unsigned long long* fresh) {
-    const int tid = threadIdx.x;
+constexpr int kCand = 256;   // candidates a group's list holds
+
+// A value that at least k of the group's maxima (one in each of `values`, over `lanes` neighbouring lanes of a wave) reach and few more
+// do: at least k classes reach it then, so no class below it is among the best k.  Bisection between the least finite maximum and
+// the largest; where ties or the step limit stop it early the value is lower than it could be, never too high.
+template <int Q>
+__device__ __forceinline__ float top_threshold(const float (&v)[Q], int k, int lanes) {
+    float lo = INFINITY, hi = -INFINITY;
+    int finite = 0;
+#pragma unroll
+    for (int q = 0; q < Q; ++q)
+        if (v[q] > -INFINITY) {
+            lo = fminf(lo, v[q]);
+            hi = fmaxf(hi, v[q]);
+            ++finite;
+        }
+    for (int off = lanes / 2; off > 0; off >>= 1) {
+        lo = fminf(lo, __shfl_xor(lo, off, 64));
+        hi = fmaxf(hi, __shfl_xor(hi, off, 64));
+        finite += __shfl_xor(finite, off, 64);
+    }
+    if (finite <= k) return -INFINITY;
+    const int enough = k + k / 4 + 1;
+    int reached = finite;
+    for (int it = 0; it < 24 && __any(reached > enough); ++it) {   // (lanes of other cases may still be at it)
+        const float mid = 0.5f * lo + 0.5f * hi;
+        int count = 0;
+#pragma unroll
+        for (int q = 0; q < Q; ++q) count += v[q] >= mid;
+        for (int off = lanes / 2; off > 0; off >>= 1) count += __shfl_xor(count, off, 64);
+        if (reached > enough) {
+            if (count >= k) {
+                lo = mid;
+                reached = count;
+            } else hi = mid;
+        }
+    }
+    return lo;
+}
+
+// The k largest keys of classes [from, to) in one walk over them in order: THREADS classes at a time against the k-th best so far;
+// what beats it joins the list, which is ordered again by counting, for each key, the larger ones.  Any number of ties, any order; used
+// where the candidate list overflows.  best: MC_MAX_TOP keys, fresh: THREADS keys of LDS.
+template <int THREADS, class T>
+__device__ void top_by_scan(const T* x, size_t stride, int from, int to, int k, unsigned long long* best, unsigned long long* fresh) {
+    typedef Group<THREADS> G;
+    const int tid = G::tid();
     if (tid < k) best[tid] = 0;
-    __syncthreads();
-    for (int base = 0; base < numOut; base += LT) {
+    G::sync();
+    for (int base = from; base < to; base += THREADS) {
         const int j = base + tid;
-        unsigned long long key = j < numOut ? top_key((float)x[(size_t)j * stride], j) : 0;
+        unsigned long long key = j < to ? top_key((float)x[(size_t)j * stride], j) : 0;
         if (key <= best[k - 1]) key = 0;
-        if (!__syncthreads_or(key != 0)) continue;
+        if (!G::any(key != 0)) continue;
         fresh[tid] = key;
         const unsigned long long mine = tid < k ? best[tid] : 0;
-        __syncthreads();
+        G::sync();
         int rank = 0, mineRank = 0;
-        for (int i = 0; i < LT; ++i) {
+#pragma unroll 4
+        for (int i = 0; i < THREADS; ++i) {
             rank += fresh[i] > key;
             mineRank += fresh[i] > mine;
         }
         for (int i = 0; i < k; ++i) rank += best[i] > key;
-        __syncthreads();
+        G::sync();
         if (mine && tid + mineRank < k) best[tid + mineRank] = mine;
         if (key && rank < k) best[rank] = key;
+        G::sync();
+    }
+}
+
+// Orders `count` distinct keys by counting, for each, the larger ones, and gives (rank, key) to `put` for the first k; ranks from
+// count on get key 0.
+template <class F>
+__device__ __forceinline__ void rank_keys(const unsigned long long* keys, int count, int k, int tid, int threads, F put) {
+    for (int i = tid; i < count; i += threads) {
+        const unsigned long long key = keys[i];
+        int rank = 0;
+        for (int c = 0; c < count; ++c) rank += keys[c] > key;
+        if (rank < k) put(rank, key);
+    }
+    for (int r = count + tid; r < k; r += threads) put(r, 0);
+}
+
+// ---------------------------------------------------------------- a case's results
+struct CaseStats { float m, logSum, log2Sum; };
+
+// (m, s, w) of all classes -> the outputs of case n; labelLogit: the label's logit, if there is a label.
+__device__ __forceinline__ CaseStats case_stats(float m, float s) {
+    const bool empty = s == 0.f;   // every class is ruled out
+    const float l2 = empty ? 0.f : log2f(s);
+    return {s != s && m == -INFINITY ? s : m, l2 * kLn2, l2};
+}
+__device__ __forceinline__ float log_prob(float x, const CaseStats& c) { return x == -INFINITY && c.logSum == c.logSum ? x : (x - c.m) - c.logSum; }
+__device__ __forceinline__ void write_case(const LogProbArgs& a, int n, const CaseStats& c, float s, float w, int label, float labelLogit) {
+    if (a.maxAndLogSum) {
+        a.maxAndLogSum[n] = c.m;
+        a.maxAndLogSum[(size_t)a.numCases + n] = c.logSum;
+    }
+    if (a.entropy) a.entropy[n] = s == 0.f ? 0.f : kLn2 * (c.log2Sum - w / s);
+    if (a.labelLogProbs) a.labelLogProbs[n] = label < 0 ? 0.f : log_prob(labelLogit, c);
+}
+__device__ __forceinline__ void write_top(const LogProbArgs& a, int n, int rank, unsigned long long key, const CaseStats& c) {
+    a.topClasses[(size_t)rank * a.numCases + n] = key ? key_class(key) : -1;
+    a.topLogProbs[(size_t)rank * a.numCases + n] = key ? log_prob(key_logit(key), c) : -INFINITY;
+}
+
+// The largest of x(0) ... x(COUNT - 1), NaN left out, two a step.  (As asm: the compiler would first quieten every operand, one more
+// instruction each.)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+template <int COUNT, class F>
+__device__ __forceinline__ float max_of(F x) {
+    if (COUNT == 1) return x(0);
+    float r = COUNT == 2 ? max3(x(0), x(1), x(1)) : max3(x(0), x(1), x(COUNT > 2 ? 2 : 0));
+#pragma unroll
+    for (int i = 3; i < COUNT; i += 2) r = max3(r, x(i), x(i + 1 < COUNT ? i + 1 : i));
+    return r;
+}
+
+// t_j = (x_j - m) log2 e as fma(x_j, scale, -c), c = m log2 e as rounded; what the rounding of c moved every t by is known (another fma)
+// and taken back once for all.  Logits of kHuge and more are equal to m or so far below it that 2^t is 0; there any scale does that does
+// not overflow.  m = -inf leaves every t at -inf.
+struct Shift { float scale, c; };
+__device__ __forceinline__ Shift shift_for(float m) {
+    const bool huge = fabsf(m) >= kHuge && m != -INFINITY;
+    const float scale = huge ? 5.4210109e-20f : kLog2e;   // 2^-64
+    return {scale, fmaxf(m, huge ? m : -kHuge) * scale};
+}
+__device__ __forceinline__ void take_back(float m, float& s, float& w) {
+    if (fabsf(m) >= kHuge) return;
+    const float c = m * kLog2e, d = fmaf(m, kLog2e, -c), f = __builtin_amdgcn_exp2f(-d);
+    w = (w - d * s) * f;
+    s *= f;
+}
+// s and w of x(0) ... x(COUNT - 1).  A t of -inf is a ruled-out class: its 2^t is 0 and so has to be its t 2^t.
+template <bool ENT, int COUNT, class F>
+__device__ __forceinline__ void sums_of(F x, Shift h, float& s, float& w) {
+    s = w = 0.f;
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) {
+        const float t = fmaf(x(i), h.scale, -h.c), e = __builtin_amdgcn_exp2f(t);
+        s += e;
+        if (ENT) w = fmaf(e, fmaxf(t, -200.f), w);
+    }
+}
+
+// N elements of type T as the registers they were loaded into.  Elements are converted where they are used; keep() stops the compiler
+// from holding the converted values from one use to the next, which would take twice the registers for 16-bit types.
+template <class T, int N>
+struct Words {
+    static constexpr int COUNT = N * sizeof(T) < 4 ? 1 : N * sizeof(T) / 4;
+    unsigned w[COUNT];
+    struct __attribute__((packed, aligned(sizeof(T)), may_alias)) Memory { unsigned w[COUNT]; };
+    __device__ __forceinline__ void load(const T* p) {
+        if (N * sizeof(T) < 4) {   // one 16-bit element
+            unsigned short h;
+            __builtin_memcpy(&h, p, 2);
+            w[0] = h;
+            return;
+        }
+        const Memory m = *reinterpret_cast<const Memory*>(p);
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) w[i] = m.w[i];
+    }
+    __device__ __forceinline__ void fill() {   // -inf
+        const unsigned inf = sizeof(T) == 4 ? 0xff800000u : __is_same(T, _Float16) ? 0xfc00fc00u : 0xff80ff80u;
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) w[i] = inf;
+    }
+    __device__ __forceinline__ void fill_first(int n) {   // -inf in the first n of them
+        const unsigned inf = sizeof(T) == 4 ? 0xff800000u : __is_same(T, _Float16) ? 0xfc00fc00u : 0xff80ff80u;
+        constexpr int PER = sizeof(T) == 4 ? 1 : 2;
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) {
+            if (PER == 2 && n == 2 * i + 1) w[i] = (w[i] & 0xffff0000u) | (inf & 0xffffu);
+            if (n >= PER * (i + 1)) w[i] = inf;
+        }
+    }
+    __device__ __forceinline__ void set(int k, T v) {
+        unsigned short h = 0;
+        if (sizeof(T) == 4) {
+            __builtin_memcpy(&w[k], &v, sizeof(T));
+            return;
+        }
+        __builtin_memcpy(&h, &v, 2);
+        w[k / 2] = k % 2 ? (w[k / 2] & 0xffffu) | (unsigned)h << 16 : (w[k / 2] & 0xffff0000u) | h;
+    }
+    __device__ __forceinline__ float at(int k) const {
+        if (sizeof(T) == 4) return __uint_as_float(w[k]);
+        const unsigned u = w[k / 2];
+        if (__is_same(T, __bf16)) return __uint_as_float(k % 2 ? u & 0xffff0000u : u << 16);
+        const unsigned short h = (unsigned short)(k % 2 ? u >> 16 : u);
+        _Float16 v;
+        __builtin_memcpy(&v, &h, 2);
+        return (float)v;
+    }
+    __device__ __forceinline__ void keep() {
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) asm("" : "+v"(w[i]));
+    }
+};
+
+// ---------------------------------------------------------------- a case's classes side by side
+// A workgroup (or wave) takes up to THREADS * U packs of 16 bytes of one case into registers in one burst of loads, and does all the
+// rest there: the largest logit, the sums against it, the candidates for the top.
+template <class T, int THREADS, int U, bool ENT, bool TOP>
+__global__ void __launch_bounds__(LT) k_log_probs_rows(LogProbArgs a, Parts p) {
+    typedef Group<THREADS> G;
+    constexpr int V = 16 / sizeof(T), GROUPS = LT / THREADS;
+    __shared__ float shRed[GROUPS][3 * (G::WAVES > 1 ? G::WAVES : 1)];
+    __shared__ float shMax[TOP ? LT : 1];
+    __shared__ unsigned long long shCand[TOP ? GROUPS : 1][TOP ? kCand + MC_MAX_TOP : 1];
+    __shared__ int shCount[GROUPS];
+    const int group = G::index(), tid = G::tid();
+    const unsigned item = blockIdx.x * GROUPS + group, row = item / (unsigned)p.parts;
+    if (row >= (unsigned)a.numCases) return;          // (whole waves: THREADS is 64 then)
+    const int n = (int)row, lo = (int)(item - row * p.parts) * p.span;
+    const T* x = static_cast<const T*>(a.logits) + row * a.caseStride + lo;   // this part's classes: lo + j, j < len
+    const int len = min(a.numOut - lo, p.span);
+    int label = -1;
+    if (p.parts == 1 && a.labelLogProbs) label = label_of(a.labels, a.labelType, n, a.numOut);
+
+    // A pack that would reach past the end starts V before the end instead, and what it then repeats of its neighbour becomes -inf.  (A
+    // last part shorter than a pack reaches back into the part before it.)
+    Words<T, V> v[U];
+    const int first = tid * V, last = len - V, back = max(-last, 0);
+    const bool whole = THREADS == LT || a.numOut >= V;
+    if (whole) {
+        const T* from = x - back;
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u].load(from + (unsigned)(min(first + u * (THREADS * V), last) + back));
+        if (len != THREADS * U * V) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) v[u].fill_first(first + u * (THREADS * V) - last);
+        }
+    } else {   // fewer classes than a pack holds
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u].fill();
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+            if (first == 0 && k < len) v[0].set(k, x[k]);
+    }
+    const float labelLogit = label >= 0 ? (float)x[label] : 0.f;   // (one part: lo is 0)
+
+    float pm[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        pm[u] = max_of<V>([&](int k) { return v[u].at(k); });
+        v[u].keep();
+    }
+    const float mine = max_of<U>([&](int u) { return pm[u]; });
+    if (TOP) {
+        shMax[threadIdx.x] = mine;
+        if (tid == 0) shCount[group] = 0;
+    }
+    const float m = G::max(mine, shRed[group]);
+    float s, w;
+    sums_of<ENT, U * V>([&](int i) { return v[i / V].at(i % V); }, shift_for(m), s, w);
+    G::sum2(s, w, shRed[group] + G::WAVES);
+    take_back(m, s, w);
+    const CaseStats c = case_stats(m, s);
+    if (tid == 0) {
+        if (p.parts == 1) write_case(a, n, c, s, w, label, labelLogit);
+        else p.stats[item] = {m, s, w, 0.f};
+    }
+    if (!TOP) return;
+
+    G::sync();
+    float q[THREADS / 64];
+#pragma unroll
+    for (int i = 0; i < THREADS / 64; ++i) q[i] = shMax[group * THREADS + i * 64 + (threadIdx.x & 63)];
+    const float threshold = top_threshold(q, a.numTop, 64);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        if (pm[u] >= threshold) {
+            v[u].keep();
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                const float y = v[u].at(k);
+                if (y >= threshold && y > -INFINITY) {
+                    const int to = atomicAdd(&shCount[group], 1);
+                    if (to < kCand) shCand[group][to] = top_key(y, lo + (whole ? min(first + u * (THREADS * V), last) : 0) + k);
+                }
+            }
+        }
+    G::sync();
+    const int count = shCount[group];
+    const auto put = [&](int rank, unsigned long long key) {
+        if (p.parts == 1) write_top(a, n, rank, key, c);
+        else p.keys[(size_t)item * a.numTop + rank] = key;
+    };
+    if (count <= kCand) rank_keys(shCand[group], count, a.numTop, tid, THREADS, put);
+    else {
+        G::sync();
+        top_by_scan<THREADS>(x - lo, 1, lo, lo + len, a.numTop, shCand[group] + kCand, shCand[group]);
+        if (tid < a.numTop) put(tid, shCand[group][kCand + tid]);
+    }
+}
+
+// ---------------------------------------------------------------- a class's cases side by side
+// A workgroup takes 256 / G classes of G * P cases at a time, U times, into registers: lane (r, g) holds P neighbouring cases of class
+// r of each.  P states a lane are reduced over the lanes that share them, then over the waves.
+constexpr int kColCand = 96;
+// LDS of the top alternatives: the candidate lists (or what top_by_scan needs), the stretches' maxima, the counts, the thresholds
+__host__ __device__ constexpr int col_list_keys(int cases) { return cases * kColCand > LT + MC_MAX_TOP ? cases * kColCand : LT + MC_MAX_TOP; }
+constexpr size_t col_lds_bytes(int cases, int stretches) {
+    return col_list_keys(cases) * sizeof(unsigned long long) + ((size_t)cases * (stretches + 1) + 2 * cases) * sizeof(float);
+}
+template <class T, int P, int U, bool ENT, bool TOP>
+__global__ void __launch_bounds__(LT) k_log_probs_cols(LogProbArgs a, Parts p, int logG) {
+    constexpr int W = U >= 4 ? U / 4 : 1, WINDOWS = U / W;   // the top's maxima are kept for W classes at a time
+    constexpr int Q = P == 1 ? 16 : WINDOWS * P;
+    extern __shared__ unsigned long long shDyn[];
+    __shared__ float shM[4][8 * P], shS[4][8 * P], shW[4][8 * P];
+    const int G = 1 << logG, R = LT >> logG, cases = G * P;
+    const int g = threadIdx.x & (G - 1), r = threadIdx.x >> logG, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int tiles = (a.numCases + cases - 1) / cases;
+    const int tile = blockIdx.x % tiles, part = blockIdx.x / tiles;
+    // (the last lanes of the last tile step back to the last P cases, or repeat them: the same values are written twice)
+    const int n0 = min((tile * G + g) * P, a.numCases - P);
+    const int lo = part * p.span, hi = min(a.numOut - lo, p.span) + lo;
+    const T* x = static_cast<const T*>(a.logits) + (size_t)n0 * (P == 1 ? a.caseStride : 1);
+
+    Words<T, P> v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        v[u].load(x + (size_t)min(lo + u * R + r, hi - 1) * a.classStride);
+    }
+    if (hi - lo != U * R) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (lo + u * R + r >= hi) v[u].fill();
+    }
+    float pm[TOP ? WINDOWS : 1][P], m[P], s[P], w[P];
+#pragma unroll
+    for (int k = 0; k < P; ++k) {
+        m[k] = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < WINDOWS; ++i) {
+            const float y = max_of<W>([&](int u) { return v[i * W + u].at(k); });
+            if (TOP) pm[i][k] = y;
+            m[k] = fmaxf(m[k], y);
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u].keep();
+    // TOP: the maxima of WINDOWS * R stretches for each case, [case][stretch]
+    float* shSeg = reinterpret_cast<float*>(shDyn + col_list_keys(cases));
+    int* shCount = reinterpret_cast<int*>(shSeg + cases * (WINDOWS * R + 1));
+    float* shTau = reinterpret_cast<float*>(shCount + cases);
+    if (TOP) {
+#pragma unroll
+        for (int k = 0; k < P; ++k)
+#pragma unroll
+            for (int i = 0; i < WINDOWS; ++i) shSeg[(g * P + k) * (WINDOWS * R + 1) + i * R + r] = pm[i][k];
+        if ((int)threadIdx.x < cases) shCount[threadIdx.x] = 0;
+    }
+#pragma unroll
+    for (int k = 0; k < P; ++k) {
+        for (int off = 32; off >= G; off >>= 1) m[k] = fmaxf(m[k], __shfl_xor(m[k], off, 64));
+        if (lane < G) shM[wave][g * P + k] = m[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < P; ++k) {
+        m[k] = fmaxf(fmaxf(shM[0][g * P + k], shM[1][g * P + k]), fmaxf(shM[2][g * P + k], shM[3][g * P + k]));
+        sums_of<ENT, U>([&](int i) { return v[i].at(k); }, shift_for(m[k]), s[k], w[k]);
+        for (int off = 32; off >= G; off >>= 1) {
+            s[k] += __shfl_xor(s[k], off, 64);
+            if (ENT) w[k] += __shfl_xor(w[k], off, 64);
+        }
+        if (lane < G) {
+            shS[wave][g * P + k] = s[k];
+            shW[wave][g * P + k] = w[k];
+        }
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < cases) {
+        const int cc = threadIdx.x, n = min((tile * G + cc / P) * P, a.numCases - P) + cc % P;
+        float M = fmaxf(fmaxf(shM[0][cc], shM[1][cc]), fmaxf(shM[2][cc], shM[3][cc]));
+        float S = shS[0][cc] + shS[1][cc] + shS[2][cc] + shS[3][cc], Wt = shW[0][cc] + shW[1][cc] + shW[2][cc] + shW[3][cc];
+        take_back(M, S, Wt);
+        if (p.parts == 1) {
+            const CaseStats c = case_stats(M, S);
+            const int label = a.labelLogProbs ? label_of(a.labels, a.labelType, n, a.numOut) : -1;
+            const float labelLogit = label >= 0 ? (float)static_cast<const T*>(a.logits)[(size_t)label * a.classStride + (size_t)n * a.caseStride] : 0.f;
+            write_case(a, n, c, S, Wt, label, labelLogit);
+            if (TOP) {
+                shS[0][cc] = c.logSum;   // (read by its own thread only until the next barrier)
+                shM[0][cc] = c.m;
+            }
+        } else p.stats[(size_t)n * p.parts + part] = {M, S, Wt, 0.f};
+    }
+    if (!TOP) return;
+
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u].keep();
+    // thresholds: `lanes` neighbouring lanes share a case's maxima
+    const int lanes = min(64, LT / cases), owner = threadIdx.x / lanes, sub = threadIdx.x % lanes, stretches = WINDOWS * R;
+    {
+        float q[Q];
+#pragma unroll
+        for (int i = 0; i < Q; ++i) {
+            const int at = sub + i * lanes;
+            q[i] = owner < cases && at < stretches ? shSeg[owner * (stretches + 1) + at] : -INFINITY;
+        }
+        const float tau = top_threshold(q, a.numTop, lanes);
+        if (owner < cases && sub == 0) shTau[owner] = tau;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < P; ++k) {
+        const float tau = shTau[g * P + k];
+#pragma unroll
+        for (int i = 0; i < WINDOWS; ++i)
+            if (pm[i][k] >= tau) {
+#pragma unroll
+                for (int u = 0; u < W; ++u) {
+                    const float y = v[i * W + u].at(k);
+                    if (y >= tau && y > -INFINITY) {
+                        const int to = atomicAdd(&shCount[g * P + k], 1);
+                        if (to < kColCand) shDyn[(g * P + k) * kColCand + to] = top_key(y, lo + (i * W + u) * R + r);
+                    }
+                }
+            }
+    }
+    __syncthreads();
+    const auto put = [&](int cc, int rank, unsigned long long key) {
+        const int n = min((tile * G + cc / P) * P, a.numCases - P) + cc % P;
+        if (p.parts == 1) write_top(a, n, rank, key, CaseStats{shM[0][cc], shS[0][cc], 0.f});
+        else p.keys[((size_t)n * p.parts + part) * a.numTop + rank] = key;
+    };
+    if (owner < cases && shCount[owner] <= kColCand)
+        rank_keys(shDyn + owner * kColCand, shCount[owner], a.numTop, sub, lanes, [&](int rank, unsigned long long key) { put(owner, rank, key); });
+    __syncthreads();
+    for (int cc = 0; cc < cases; ++cc) {   // lists that overflowed: the lists' memory is free by now
+        if (shCount[cc] <= kColCand) continue;
+        const int n = min((tile * G + cc / P) * P, a.numCases - P) + cc % P;
+        top_by_scan<LT>(static_cast<const T*>(a.logits) + (size_t)n * a.caseStride, a.classStride, lo, hi, a.numTop, shDyn + LT, shDyn);
+        if ((int)threadIdx.x < a.numTop) put(cc, threadIdx.x, shDyn[LT + threadIdx.x]);
         __syncthreads();
     }
 }
 
-template <class T>
-__global__ void __launch_bounds__(LT) k_log_probs(LogProbArgs a) {
-    __shared__ float sh[LT / 64];
-    __shared__ unsigned long long best[MC_MAX_TOP], fresh[LT];
-    for (int n = blockIdx.x; n < a.numCases; n += gridDim.x) {
-        const T* x = static_cast<const T*>(a.logits) + (size_t)n * a.caseStride;
-        float m = -INFINITY;
-        for (int j = threadIdx.x; j < a.numOut; j += LT) m = fmaxf(m, (float)x[(size_t)j * a.classStride]);
-        m = block_max(m, sh);
-        float s = 0.f, w = 0.f;
-        for (int j = threadIdx.x; j < a.numOut; j += LT) {
-            const float v = (float)x[(size_t)j * a.classStride];
-            const float t = v == -INFINITY ? -INFINITY : v - m;
-            const float e = expf(t);
-            s += e;
-            w += e * fmaxf(t, -200.f);   // e is 0 there
+// ---------------------------------------------------------------- joining the parts of a case
+constexpr int kJoinCand = 1024;
+template <class T, int THREADS>
+__global__ void __launch_bounds__(LT) k_log_probs_join(LogProbArgs a, Parts p) {
+    typedef Group<THREADS> G;
+    constexpr int GROUPS = LT / THREADS, CAND = THREADS == 64 ? kJoinCand / 4 : kJoinCand;
+    __shared__ float shRed[GROUPS][3 * G::WAVES];
+    __shared__ unsigned long long shCand[GROUPS][CAND];
+    __shared__ int shCount[GROUPS];
+    const int group = G::index(), tid = G::tid();
+    const size_t row = (size_t)blockIdx.x * GROUPS + group;
+    if (row >= (size_t)a.numCases) return;
+    const int n = (int)row;
+    const int label = a.labelLogProbs ? label_of(a.labels, a.labelType, n, a.numOut) : -1;
+    const Part* stats = p.stats + row * p.parts;
+    const float labelLogit = label >= 0 ? (float)static_cast<const T*>(a.logits)[(size_t)label * a.classStride + row * a.caseStride] : 0.f;
+    if (tid == 0) shCount[group] = 0;
+    float m = -INFINITY;
+    for (int i = tid; i < p.parts; i += THREADS) m = fmaxf(m, stats[i].m);
+    m = G::max(m, shRed[group]);
+    float s = 0.f, w = 0.f;
+    for (int i = tid; i < p.parts; i += THREADS) {
+        const Part q = stats[i];
+        const float d = q.m == m ? 0.f : (q.m - m) * kLog2e, f = __builtin_amdgcn_exp2f(d);
+        s += q.s * f;
+        w += fmaf(fmaxf(d, -200.f), q.s, q.w) * f;
+    }
+    G::sum2(s, w, shRed[group] + G::WAVES);
+    const CaseStats c = case_stats(m, s);
+    if (tid == 0) write_case(a, n, c, s, w, label, labelLogit);
+    if (!a.numTop) return;
+
+    // candidates: keys that reach a value that numTop parts' best keys reach
+    const unsigned long long* keys = p.keys + row * p.parts * a.numTop;
+    float threshold = -INFINITY;
+    if (p.parts > a.numTop) {
+        constexpr int Q = 8;
+        float q[Q];
+        const int parts = min(p.parts, 64 * Q);   // (beyond: the first ones' threshold holds too)
+#pragma unroll
+        for (int i = 0; i < Q; ++i) {
+            const int at = (threadIdx.x & 63) + 64 * i;
+            const unsigned long long key = at < parts ? keys[(size_t)at * a.numTop] : 0;
+            q[i] = key ? key_logit(key) : -INFINITY;
         }
-        s = block_sum(s, sh);
-        w = block_sum(w, sh);
-        const bool empty = s == 0.f;   // every class is ruled out
-        const float logSum = empty ? 0.f : logf(s);
-        if (threadIdx.x == 0) {
-            if (a.maxAndLogSum) {
-                a.maxAndLogSum[n] = s != s && m == -INFINITY ? s : m;
-                a.maxAndLogSum[a.numCases + n] = logSum;
-            }
-            if (a.entropy) a.entropy[n] = empty ? 0.f : logSum - w / s;
-            if (a.labelLogProbs) {
-                const int y = label_of(a.labels, a.labelType, n, a.numOut);
-                const float v = y < 0 ? 0.f : (float)x[(size_t)y * a.classStride];
-                a.labelLogProbs[n] = y < 0 ? 0.f : v == -INFINITY && s == s ? v : (v - m) - logSum;
-            }
+        threshold = top_threshold(q, a.numTop, 64);
+    }
+    const int total = p.parts * a.numTop;
+    G::sync();
+    for (int i = tid; i < total; i += THREADS) {
+        const unsigned long long key = keys[i];
+        if (key && key_logit(key) >= threshold) {
+            const int to = atomicAdd(&shCount[group], 1);
+            if (to < CAND) shCand[group][to] = key;
         }
-        if (a.numTop) {
-            top_by_scan(x, a.classStride, a.numOut, a.numTop, best, fresh);
-            if ((int)threadIdx.x < a.numTop) {
-                const unsigned long long key = best[threadIdx.x];
-                a.topClasses[(size_t)threadIdx.x * a.numCases + n] = key ? key_class(key) : -1;
-                a.topLogProbs[(size_t)threadIdx.x * a.numCases + n] = key ? (key_logit(key) - m) - logSum : -INFINITY;
-            }
-            __syncthreads();
+    }
+    G::sync();
+    const int count = shCount[group];
+    if (count <= CAND) {
+        rank_keys(shCand[group], count, a.numTop, tid, THREADS, [&](int rank, unsigned long long key) { write_top(a, n, rank, key, c); });
+        return;
+    }
+    // more ties than the list holds: the best, then the best below it, and so on
+    unsigned long long last = ~0ull;
+    for (int r = 0; r < a.numTop; ++r) {
+        unsigned long long best = 0;
+        for (int i = tid; i < total; i += THREADS) {
+            const unsigned long long key = keys[i];
+            if (key < last && key > best) best = key;
         }
+        for (int off = 32; off > 0; off >>= 1) best = std::max(best, __shfl_xor(best, off, 64));
+        if (G::WAVES > 1) {
+            G::sync();
+            if ((threadIdx.x & 63) == 0) shCand[group][threadIdx.x >> 6] = best;
+            G::sync();
+            for (int i = 0; i < G::WAVES; ++i) best = std::max(best, shCand[group][i]);
+        }
+        if (tid == 0) write_top(a, n, r, best, c);
+        last = best;
     }
 }
 
+// ---------------------------------------------------------------- the gradient
 struct LogProbGradArgs {
     const void* logits;
     size_t classStride, caseStride;
@@ -148,24 +650,129 @@ struct LogProbGradArgs {
     int add;
 };
 
-template <class T>
-__global__ void __launch_bounds__(LT) k_log_probs_grad(LogProbGradArgs a) {
-    const size_t count = (size_t)a.numCases * a.numOut;
-    for (size_t i = (size_t)blockIdx.x * LT + threadIdx.x; i < count; i += (size_t)gridDim.x * LT) {
-        const int n = a.classStride == 1 ? (int)(i / a.numOut) : (int)(i % a.numCases), j = a.classStride == 1 ? (int)(i % a.numOut) : (int)(i / a.numCases);
-        const float m = a.maxAndLogSum[n], logSum = a.maxAndLogSum[a.numCases + n];
-        const float v = (float)static_cast<const T*>(a.logits)[j * a.classStride + n * a.caseStride];
-        float d = 0.f;
-        if (m != -INFINITY) {
-            const float lp = (v - m) - logSum, p = expf(lp);
-            const int y = a.scaleLabel != 0.f ? label_of(a.labels, a.labelType, n, a.numOut) : -1;
-            const float g = y >= 0 ? a.scaleLabel * (a.gradLabel ? a.gradLabel[n] : 1.f) : 0.f;
-            d = (a.scaleLogZ != 0.f ? a.scaleLogZ * (a.gradLogZ ? a.gradLogZ[n] : 1.f) : 0.f) - g;
-            if (a.scaleEntropy != 0.f) d -= a.scaleEntropy * (a.gradEntropy ? a.gradEntropy[n] : 1.f) * (fmaxf(lp, -200.f) + a.entropy[n]);
-            d = p * d + (j == y ? g : 0.f);
+// d_j = p_j (A - h (ln p_j + H)) + [j = y] a
+struct CaseGrad { float m, logSum, A, h, H, a; int y; };
+template <bool ENT>
+__device__ __forceinline__ CaseGrad case_grad(const LogProbGradArgs& g, int n) {
+    CaseGrad c;
+    c.m = g.maxAndLogSum[n];
+    c.logSum = g.maxAndLogSum[(size_t)g.numCases + n];
+    c.y = g.scaleLabel != 0.f ? label_of(g.labels, g.labelType, n, g.numOut) : -1;
+    c.a = c.y >= 0 ? g.scaleLabel * (g.gradLabel ? g.gradLabel[n] : 1.f) : 0.f;
+    c.A = (g.scaleLogZ != 0.f ? g.scaleLogZ * (g.gradLogZ ? g.gradLogZ[n] : 1.f) : 0.f) - c.a;
+    c.h = ENT ? g.scaleEntropy * (g.gradEntropy ? g.gradEntropy[n] : 1.f) : 0.f;
+    c.H = ENT ? g.entropy[n] : 0.f;
+    if (c.m == -INFINITY) {   // every class is ruled out: p = 0 throughout, and the label's term goes too
+        c.m = c.logSum = c.a = 0.f;
+        c.y = -1;
+    }
+    return c;
+}
+template <bool ENT>
+__device__ __forceinline__ float grad_of(float x, const CaseGrad& c) {
+    const float lp = (x - c.m) - c.logSum, p = __builtin_amdgcn_exp2f(lp * kLog2e);
+    return ENT ? p * fmaf(-c.h, fmaxf(lp, -200.f) + c.H, c.A) : p * c.A;
+}
+
+template <class T, int THREADS, int U, bool ENT>
+__global__ void __launch_bounds__(LT) k_log_probs_grad_rows(LogProbGradArgs g, int parts) {
+    constexpr int V = 16 / sizeof(T), GROUPS = LT / THREADS;
+    const size_t item = (size_t)blockIdx.x * GROUPS + threadIdx.x / THREADS;
+    const size_t row = item / parts;
+    if (row >= (size_t)g.numCases) return;
+    const int lo = (int)(item - row * parts) * (THREADS * U * V);
+    const T* x = static_cast<const T*>(g.logits) + row * g.caseStride;
+    T* out = static_cast<T*>(g.target) + row * g.targetCaseStride;
+    const int first = lo + (threadIdx.x & (THREADS - 1)) * V;
+    Pack<T, V> v[U], t[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int j = first + u * (THREADS * V);
+        if (j <= g.numOut - V) v[u] = load_pack<T, V>(x + j);
+        else {
+#pragma unroll
+            for (int k = 0; k < V; ++k) v[u].v[k] = j < g.numOut - k ? x[j + k] : (T)0.f;
         }
-        T* out = static_cast<T*>(a.target) + (j * a.targetClassStride + n * a.targetCaseStride);
-        *out = (T)(a.add ? (float)*out + d : d);
+        if (g.add) {
+            if (j <= g.numOut - V) t[u] = load_pack<T, V>(out + j);
+            else {
+#pragma unroll
+                for (int k = 0; k < V; ++k) t[u].v[k] = j < g.numOut - k ? out[j + k] : (T)0.f;
+            }
+        }
+    }
+    const CaseGrad c = case_grad<ENT>(g, (int)row);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int j = first + u * (THREADS * V);
+        Pack<T, V> d;
+        const bool here = (unsigned)(c.y - j) < (unsigned)V;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            float y = grad_of<ENT>((float)v[u].v[k], c);
+            if (here && c.y == j + k) y += c.a;
+            if (g.add) y += (float)t[u].v[k];
+            d.v[k] = (T)y;
+        }
+        if (j <= g.numOut - V) store_pack<T, V>(out + j, d);
+        else {
+#pragma unroll
+            for (int k = 0; k < V; ++k)
+                if (j < g.numOut - k) out[j + k] = d.v[k];
+        }
+    }
+}
+
+template <class T, int P, int U, bool ENT>
+__global__ void __launch_bounds__(LT) k_log_probs_grad_cols(LogProbGradArgs g, int logG) {
+    const int G = 1 << logG, R = LT >> logG;
+    const int gg = threadIdx.x & (G - 1), r = threadIdx.x >> logG;
+    const int tiles = (g.numCases + G * P - 1) / (G * P);
+    const int n0 = (blockIdx.x % tiles * G + gg) * P;
+    const int j0 = (int)(blockIdx.x / tiles) * (R * U) + r;
+    if (n0 >= g.numCases) return;
+    const T* x = static_cast<const T*>(g.logits) + (size_t)n0 * (P == 1 ? g.caseStride : 1);
+    T* out = static_cast<T*>(g.target) + (size_t)n0 * (P == 1 ? g.targetCaseStride : 1);
+    const bool whole = n0 <= g.numCases - P;
+    Pack<T, P> v[U], t[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int j = j0 + u * R;
+        if (j >= g.numOut) continue;
+        const T* from = x + (size_t)j * g.classStride;
+        const T* prev = out + (size_t)j * g.targetClassStride;
+        if (whole) {
+            v[u] = load_pack<T, P>(from);
+            if (g.add) t[u] = load_pack<T, P>(prev);
+        } else {
+#pragma unroll
+            for (int k = 0; k < P; ++k) {
+                v[u].v[k] = n0 < g.numCases - k ? from[k] : (T)0.f;
+                if (g.add) t[u].v[k] = n0 < g.numCases - k ? prev[k] : (T)0.f;
+            }
+        }
+    }
+    CaseGrad c[P];
+#pragma unroll
+    for (int k = 0; k < P; ++k) c[k] = case_grad<ENT>(g, min(n0 + k, g.numCases - 1));
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int j = j0 + u * R;
+        if (j >= g.numOut) continue;
+        T* to = out + (size_t)j * g.targetClassStride;
+        Pack<T, P> d;
+#pragma unroll
+        for (int k = 0; k < P; ++k) {
+            float y = grad_of<ENT>((float)v[u].v[k], c[k]) + (j == c[k].y ? c[k].a : 0.f);
+            if (g.add) y += (float)t[u].v[k];
+            d.v[k] = (T)y;
+        }
+        if (whole) store_pack<T, P>(to, d);
+        else {
+#pragma unroll
+            for (int k = 0; k < P; ++k)
+                if (n0 < g.numCases - k) to[k] = d.v[k];
+        }
     }
 }
 
@@ -188,23 +795,124 @@ int check_labels(const char* what, const void* labels, int labelType, int numOut
     return MC_OK;
 }
 
+// ---------------------------------------------------------------- how a call is cut up
+// Logits with a case's classes side by side: up to 64 * 4 packs of 16 bytes a wave takes a case, beyond a workgroup, and a case is split
+// where it is longer than 256 * 16 packs or where there are too few cases to fill the device.  Class-major logits: see below.
+struct Plan {
+    bool rows;
+    int threads;   // rows: of a group
+    int P, logG;   // cols: cases of a lane, lanes of a class
+    int U;
+    Parts parts;
+    size_t blocks, bytes;
+};
+Plan plan_log_probs(int type, int kinds, int numCases, int numOut, int numTop) {
+    Plan p{};
+    const int V = 16 / elem_size(type), cus = num_cus();
+    p.rows = kinds & BY_CASE;
+    p.parts.parts = 1;
+    if (p.rows) {
+        if (numOut <= 64 * V * 4) {
+            p.threads = 64;
+            p.U = numOut <= 64 * V ? 1 : 4;
+            p.parts.span = numOut;
+            p.blocks = ceil_div(numCases, LT / 64);
+        } else {
+            p.threads = LT;
+            for (p.U = 16; p.U > 1 && (size_t)numCases * ceil_div(numOut, LT * V * p.U) < 2 * (size_t)cus; p.U /= 4) {}
+            p.parts.parts = ceil_div(numOut, LT * V * p.U);
+            p.parts.span = ceil_div(ceil_div(numOut, p.parts.parts), V) * V;
+            p.parts.parts = ceil_div(numOut, p.parts.span);
+            p.blocks = (size_t)numCases * p.parts.parts;
+        }
+    } else {
+        p.P = numTop ? 4 : V;
+        if (numCases < p.P) p.P = 1;
+        while (p.logG < 3 && (p.P << p.logG) < numCases) ++p.logG;
+        const int R = LT >> p.logG, tiles = ceil_div(numCases, p.P << p.logG);
+        for (p.U = 16; p.U > 1 && (numOut <= R * (p.U / 4) || (size_t)tiles * ceil_div(numOut, R * p.U) < 2 * (size_t)cus); p.U /= 4) {}
+        p.parts.span = R * p.U;
+        p.parts.parts = ceil_div(numOut, p.parts.span);
+        p.blocks = (size_t)tiles * p.parts.parts;
+    }
+    if (p.parts.parts > 1) p.bytes = (size_t)numCases * p.parts.parts * (sizeof(Part) + numTop * sizeof(unsigned long long));
+    return p;
+}
+
+template <class T, bool ENT, bool TOP>
+void launch_rows(const Plan& p, const LogProbArgs& a, hipStream_t s) {
+    const dim3 grid((unsigned)p.blocks), block(LT);
+    if (p.threads == 64) {
+        if (p.U == 1) hipLaunchKernelGGL((k_log_probs_rows<T, 64, 1, ENT, TOP>), grid, block, 0, s, a, p.parts);
+        else hipLaunchKernelGGL((k_log_probs_rows<T, 64, 4, ENT, TOP>), grid, block, 0, s, a, p.parts);
+    } else if (p.U == 1) hipLaunchKernelGGL((k_log_probs_rows<T, LT, 1, ENT, TOP>), grid, block, 0, s, a, p.parts);
+    else if (p.U == 4) hipLaunchKernelGGL((k_log_probs_rows<T, LT, 4, ENT, TOP>), grid, block, 0, s, a, p.parts);
+    else hipLaunchKernelGGL((k_log_probs_rows<T, LT, 16, ENT, TOP>), grid, block, 0, s, a, p.parts);
+}
+template <class T, int P, bool ENT, bool TOP>
+void launch_cols(const Plan& p, const LogProbArgs& a, hipStream_t s) {
+    const dim3 grid((unsigned)p.blocks), block(LT);
+    const size_t lds = TOP ? col_lds_bytes(P << p.logG, std::min(p.U, 4) * (LT >> p.logG)) : 0;
+    if (p.U == 1) hipLaunchKernelGGL((k_log_probs_cols<T, P, 1, ENT, TOP>), grid, block, lds, s, a, p.parts, p.logG);
+    else if (p.U == 4) hipLaunchKernelGGL((k_log_probs_cols<T, P, 4, ENT, TOP>), grid, block, lds, s, a, p.parts, p.logG);
+    else hipLaunchKernelGGL((k_log_probs_cols<T, P, 16, ENT, TOP>), grid, block, lds, s, a, p.parts, p.logG);
+}
+template <class T, bool ENT, bool TOP>
+void launch_log_probs(const Plan& p, const LogProbArgs& a, hipStream_t s) {
+    if (p.rows) launch_rows<T, ENT, TOP>(p, a, s);
+    else if (p.P == 1) launch_cols<T, 1, ENT, TOP>(p, a, s);
+    else launch_cols<T, TOP ? 4 : 16 / (int)sizeof(T), ENT, TOP>(p, a, s);
+    if (p.parts.parts == 1) return;
+    // a wave joins up to 64 parts; few cases of many parts take a workgroup each
+    if (p.parts.parts <= 16) hipLaunchKernelGGL((k_log_probs_join<T, 64>), dim3(ceil_div(a.numCases, LT / 64)), dim3(LT), 0, s, a, p.parts);
+    else hipLaunchKernelGGL((k_log_probs_join<T, LT>), dim3(a.numCases), dim3(LT), 0, s, a, p.parts);
+}
+
+template <class T, bool ENT>
+void launch_grad(const LogProbGradArgs& g, bool rows, hipStream_t s) {
+    constexpr int V = 16 / (int)sizeof(T);
+    const dim3 block(LT);
+    if (rows) {
+        if (g.numOut <= 64 * V * 4) {
+            const dim3 grid(ceil_div(g.numCases, LT / 64));
+            if (g.numOut <= 64 * V) hipLaunchKernelGGL((k_log_probs_grad_rows<T, 64, 1, ENT>), grid, block, 0, s, g, 1);
+            else hipLaunchKernelGGL((k_log_probs_grad_rows<T, 64, 4, ENT>), grid, block, 0, s, g, 1);
+        } else {
+            const int parts = ceil_div(g.numOut, LT * V * 4);
+            hipLaunchKernelGGL((k_log_probs_grad_rows<T, LT, 4, ENT>), dim3((unsigned)((size_t)g.numCases * parts)), block, 0, s, g, parts);
+        }
+        return;
+    }
+    int logG = 0;
+    const int P = g.numCases < V ? 1 : V;
+    while (logG < 4 && (P << logG) < g.numCases) ++logG;
+    const unsigned blocks = (unsigned)((size_t)ceil_div(g.numCases, P << logG) * ceil_div(g.numOut, (LT >> logG) * 4));
+    if (P == 1) hipLaunchKernelGGL((k_log_probs_grad_cols<T, 1, 4, ENT>), dim3(blocks), block, 0, s, g, logG);
+    else hipLaunchKernelGGL((k_log_probs_grad_cols<T, V, 4, ENT>), dim3(blocks), block, 0, s, g, logG);
+}
+
 }  // namespace
 }  // namespace mc
 using namespace mc;
 
 extern "C" {
 
-size_t mc_log_probs_workspace_bytes(int type, long long classStride, long long caseStride, int numCases, int numOut, int numTop) { return 0; }
+size_t mc_log_probs_workspace_bytes(int type, long long classStride, long long caseStride, int numCases, int numOut, int numTop) {
+    if (!float_type(type) || numCases <= 0 || numOut <= 0 || numOut > kMaxOut || numTop < 0 || numTop > MC_MAX_TOP) return 0;
+    const int kinds = layout_kinds(classStride, caseStride, numCases, numOut);
+    return kinds ? plan_log_probs(type, kinds, numCases, numOut, numTop).bytes : 0;
+}
 
 int mc_log_probs(const void* logits, int type, long long classStride, long long caseStride, const void* labels, int labelType, int numCases, int numOut,
                  float* labelLogProbs, float* entropy, float* maxAndLogSum, int* topClasses, float* topLogProbs, int numTop, void* workspace,
                  size_t workspaceBytes, mcStream_t s) {
-    MC_REQUIRE(numCases >= 0 && numOut > 0, "mc_log_probs: %d cases of %d classes", numCases, numOut);
+    MC_REQUIRE(numCases >= 0 && numOut > 0 && numOut <= kMaxOut, "mc_log_probs: %d cases of %d classes", numCases, numOut);
     MC_REQUIRE(float_type(type), "mc_log_probs: unknown element type %d", type);
     MC_REQUIRE(numTop >= 0 && numTop <= MC_MAX_TOP, "mc_log_probs: numTop must be in [0, %d]", MC_MAX_TOP);
     if (numCases == 0) return MC_OK;
     MC_REQUIRE(logits && (size_t)logits % elem_size(type) == 0, "mc_log_probs: logits are null or not aligned to their elements");
-    MC_REQUIRE(layout_kinds(classStride, caseStride, numCases, numOut), "mc_log_probs: " MC_LAYOUT_RULE);
+    const int kinds = layout_kinds(classStride, caseStride, numCases, numOut);
+    MC_REQUIRE(kinds, "mc_log_probs: " MC_LAYOUT_RULE);
     if (labelLogProbs) {
         const int rc = check_labels("mc_log_probs", labels, labelType, numOut);
         if (rc) return rc;
@@ -212,9 +920,22 @@ int mc_log_probs(const void* logits, int type, long long classStride, long long 
     MC_REQUIRE(numTop ? topClasses && topLogProbs : !topClasses && !topLogProbs, "mc_log_probs: topClasses and topLogProbs are needed exactly where numTop > 0");
     MC_REQUIRE(labelLogProbs || entropy || maxAndLogSum || numTop, "mc_log_probs: no output asked for");
     MC_REQUIRE(stream_on_current_device(s), "mc_log_probs: the stream belongs to another device than the current one");
+    Plan p = plan_log_probs(type, kinds, numCases, numOut, numTop);
+    MC_REQUIRE(p.blocks <= 0x7fffffff, "mc_log_probs: too many cases");
+    if (p.bytes && (!workspace || workspaceBytes < p.bytes || !aligned16(workspace))) {
+        set_error("mc_log_probs: workspace of %zu bytes, 16-byte aligned, needed", p.bytes);
+        return MC_EWORKSPACE;
+    }
+    p.parts.stats = static_cast<Part*>(workspace);
+    p.parts.keys = reinterpret_cast<unsigned long long*>(p.parts.stats + (p.bytes ? (size_t)numCases * p.parts.parts : 0));
     const LogProbArgs a{logits, (size_t)classStride, (size_t)caseStride, labels, labelType, numCases, numOut, labelLogProbs, entropy, maxAndLogSum,
                         topClasses, topLogProbs, numTop};
-    with_type(type, [&](auto t) { hipLaunchKernelGGL(k_log_probs<decltype(t)>, dim3(numCases < 65536 ? numCases : 65536), dim3(LT), 0, S(s), a); });
+    with_type(type, [&](auto t) {
+        typedef decltype(t) T;
+        if (numTop) launch_log_probs<T, true, true>(p, a, S(s));
+        else if (entropy) launch_log_probs<T, true, false>(p, a, S(s));
+        else launch_log_probs<T, false, false>(p, a, S(s));
+    });
     return launch_status("mc_log_probs");
 }
 
@@ -222,7 +943,7 @@ int mc_log_probs_grad(const void* logits, int type, long long classStride, long 
                       int numOut, const float* maxAndLogSum, const float* entropy, const float* gradLabel, float scaleLabel, const float* gradEntropy,
                       float scaleEntropy, const float* gradLogZ, float scaleLogZ, void* target, long long targetClassStride,
                       long long targetCaseStride, int add, mcStream_t s) {
-    MC_REQUIRE(numCases >= 0 && numOut > 0, "mc_log_probs_grad: %d cases of %d classes", numCases, numOut);
+    MC_REQUIRE(numCases >= 0 && numOut > 0 && numOut <= kMaxOut, "mc_log_probs_grad: %d cases of %d classes", numCases, numOut);
     MC_REQUIRE(float_type(type), "mc_log_probs_grad: unknown element type %d", type);
     if (numCases == 0) return MC_OK;
     MC_REQUIRE(logits && target && (size_t)logits % elem_size(type) == 0 && (size_t)target % elem_size(type) == 0,
@@ -245,8 +966,11 @@ int mc_log_probs_grad(const void* logits, int type, long long classStride, long 
     MC_REQUIRE(stream_on_current_device(s), "mc_log_probs_grad: the stream belongs to another device than the current one");
     const LogProbGradArgs a{logits, (size_t)classStride, (size_t)caseStride, labels, labelType, numCases, numOut, maxAndLogSum, entropy, gradLabel,
                             gradEntropy, gradLogZ, scaleLabel, scaleEntropy, scaleLogZ, target, (size_t)targetClassStride, (size_t)targetCaseStride, add};
-    const size_t want = ((size_t)numCases * numOut + LT - 1) / LT, cap = (size_t)num_cus() * 16;
-    with_type(type, [&](auto t) { hipLaunchKernelGGL(k_log_probs_grad<decltype(t)>, dim3((unsigned)(want < cap ? want : cap)), dim3(LT), 0, S(s), a); });
+    with_type(type, [&](auto t) {
+        typedef decltype(t) T;
+        if (scaleEntropy != 0.f) launch_grad<T, true>(a, kinds & targetKinds & BY_CASE, S(s));
+        else launch_grad<T, false>(a, kinds & targetKinds & BY_CASE, S(s));
+    });
     return launch_status("mc_log_probs_grad");
 }
 

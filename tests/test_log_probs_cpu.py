@@ -24,7 +24,7 @@ def forward(logits=P, type=0, cs=1, ns=100, labels=P, label_type=3, N=4, V=100, 
 
 
 @pytest.mark.parametrize("kw,text", [
-    (dict(V=0), "classes"), (dict(N=-1), "cases"), (dict(type=3), "element type"), (dict(type=-1), "element type"), (dict(logits=None), "logits"),
+    (dict(V=0), "classes"), (dict(V=(1 << 30) + 1, ns=1 << 31), "classes"), (dict(N=-1), "cases"), (dict(type=3), "element type"), (dict(type=-1), "element type"), (dict(logits=None), "logits"),
     (dict(logits=P + 2), "aligned"), (dict(type=2, logits=P + 1), "aligned"), (dict(cs=2, ns=100), "stride"), (dict(cs=1, ns=99), "stride"),
     (dict(cs=3, ns=1), "stride"), (dict(cs=0, ns=1), "positive"), (dict(cs=1, ns=-100), "positive"), (dict(cs=1, ns=1 << 62), "large"),
     (dict(labels=None), "labels"), (dict(labels=P + 2), "labels"), (dict(label_type=1), "MC_I32"), (dict(k=-1), "numTop"), (dict(k=33, classes=P, top=P), "numTop"),
@@ -58,6 +58,18 @@ def test_workspace_refusals():
     assert L.mc_grad_norm(P, 3, 1.0, P, None, 0, None) == -3 and "workspace" in last()
     assert L.mc_grad_norm(P, 3, 1.0, P, P, 8, None) == -3
     assert L.mc_grad_norm(P, 3, 1.0, P, P + 8, 1 << 20, None) == -3
+
+
+def test_workspace_of_split_cases():
+    L = lib()
+    size = L.mc_log_probs_workspace_bytes(2, 1, 131072, 1, 131072, 20)
+    assert size > 0
+    kw = dict(type=2, ns=131072, N=1, V=131072, classes=P, top=P, k=20)
+    assert forward(**kw) == -3 and "workspace" in last()
+    assert forward(work=P, size=size - 1, **kw) == -3 and forward(work=P + 8, size=size, **kw) == -3
+    assert L.mc_log_probs_workspace_bytes(0, 128, 1, 128, 10, 5) == 0               # short cases take one launch and no workspace
+    for bad in ((3, 1, 10, 4, 10, 0), (0, 2, 2, 4, 10, 0), (0, 1, 10, -1, 10, 0), (0, 1, 10, 4, 0, 0), (0, 1, 10, 4, 10, 33)):
+        assert L.mc_log_probs_workspace_bytes(*bad) == 0
 
 
 @pytest.mark.parametrize("args", [(None, 3, 1.0, P), (P, -1, 1.0, P), (P, 3, 0.0, P), (P, 3, -1.0, P), (P, 3, float("nan"), P), (P, 3, 1.0, None)])
