@@ -110,6 +110,8 @@ def _logits(case, gen):
 
 
 def _kernels():
+    if "mckernels" in sys.modules:      # a program imports it once
+        return sys.modules["mckernels"]
     folder = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "cuda-convnet_amd")
     here = os.path.join(os.getcwd(), "cuda-convnet_amd")
     folder = here if os.path.isdir(here) else folder
