@@ -26,35 +26,45 @@ __device__ __forceinline__ double block_sum(double v, double* sh) {
 }
 
 template <class T>
+__device__ __forceinline__ void add_square(double& acc, T x) {
+    const double d = (double)(float)x;
+    acc += d * d;
+}
+template <class T>
 __device__ __forceinline__ double span_square(const T* g, unsigned n) {
-    constexpr int V = 16 / sizeof(T);
-    double acc = 0.0;
-    const unsigned nv = n / V;
-    for (unsigned i = threadIdx.x; i < nv; i += GT) {
-        const Pack<T, V> x = load_pack<T, V>(g + (size_t)i * V);
+    constexpr int V = 16 / sizeof(T), U = 8;   // U loads in flight a thread
+    double acc[2] = {0.0, 0.0};
+    unsigned i = 0;
+    for (; i + GT * V * U <= n; i += GT * V * U) {
+        Pack<T, V> x[U];
 #pragma unroll
-        for (int k = 0; k < V; ++k) {
-            const double d = (double)(float)x.v[k];
-            acc += d * d;
-        }
+        for (int u = 0; u < U; ++u) x[u] = load_pack<T, V>(g + i + (u * GT + threadIdx.x) * V);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int k = 0; k < V; ++k) add_square(acc[k & 1], x[u].v[k]);
     }
-    for (unsigned i = nv * V + threadIdx.x; i < n; i += GT) {
-        const double d = (double)(float)g[i];
-        acc += d * d;
+    for (; i + GT * V <= n; i += GT * V) {
+        const Pack<T, V> x = load_pack<T, V>(g + i + threadIdx.x * V);
+#pragma unroll
+        for (int k = 0; k < V; ++k) add_square(acc[k & 1], x.v[k]);
     }
-    return acc;
+    for (i += threadIdx.x; i < n; i += GT) add_square(acc[0], g[i]);
+    return acc[0] + acc[1];
 }
 
 __global__ void __launch_bounds__(GT) k_grad_square(const mcGradSpan* __restrict__ spans, int numSpans, double* __restrict__ partials) {
     __shared__ double sh[GT / 64];
     double acc = 0.0;
+    mcGradSpan sp = spans[blockIdx.x];
     for (int b = blockIdx.x; b < numSpans; b += gridDim.x) {
-        const mcGradSpan sp = spans[b];
+        const mcGradSpan next = spans[min(b + (int)gridDim.x, numSpans - 1)];   // its way to memory is as long as a gradient's
         double s = 0.0;
         if (sp.gradType == MC_F32) s = span_square(static_cast<const float*>(sp.grad), sp.count);
         else if (sp.gradType == MC_F16) s = span_square(static_cast<const _Float16*>(sp.grad), sp.count);
         else s = span_square(static_cast<const __bf16*>(sp.grad), sp.count);
         acc += s * ((double)sp.scale * (double)sp.scale);
+        sp = next;
     }
     acc = block_sum(acc, sh);
     if (threadIdx.x == 0) partials[blockIdx.x] = acc;
@@ -76,16 +86,21 @@ __global__ void __launch_bounds__(GT) k_grad_factor(const double* __restrict__ p
 
 template <class T, class O>
 __device__ __forceinline__ void span_scale(const T* g, O* out, unsigned n, float f) {
-    constexpr int V = 16 / (sizeof(T) > sizeof(O) ? sizeof(T) : sizeof(O));
-    const unsigned nv = n / V;
-    for (unsigned i = threadIdx.x; i < nv; i += GT) {
-        const Pack<T, V> x = load_pack<T, V>(g + (size_t)i * V);
-        Pack<O, V> y;
+    constexpr int V = 16 / (sizeof(T) > sizeof(O) ? sizeof(T) : sizeof(O)), U = 4;
+    unsigned i = 0;
+    for (; i + GT * V * U <= n; i += GT * V * U) {
+        Pack<T, V> x[U];
 #pragma unroll
-        for (int k = 0; k < V; ++k) y.v[k] = (O)((float)x.v[k] * f);
-        store_pack<O, V>(out + (size_t)i * V, y);
+        for (int u = 0; u < U; ++u) x[u] = load_pack<T, V>(g + i + (u * GT + threadIdx.x) * V);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            Pack<O, V> y;
+#pragma unroll
+            for (int k = 0; k < V; ++k) y.v[k] = (O)((float)x[u].v[k] * f);
+            store_pack<O, V>(out + i + (u * GT + threadIdx.x) * V, y);
+        }
     }
-    for (unsigned i = nv * V + threadIdx.x; i < n; i += GT) out[i] = (O)((float)g[i] * f);
+    for (i += threadIdx.x; i < n; i += GT) out[i] = (O)((float)g[i] * f);
 }
 template <class O>
 __device__ __forceinline__ void span_zero(O* out, unsigned n) {
@@ -102,8 +117,10 @@ __device__ __forceinline__ void span_clip(const mcGradSpan& sp, float factor) {
 
 __global__ void __launch_bounds__(GT) k_clip_grads(const mcGradSpan* __restrict__ spans, int numSpans, const float* __restrict__ normAndFactor) {
     const float factor = normAndFactor[1];
-    for (int b = blockIdx.x; b < numSpans; b += gridDim.x) {
-        const mcGradSpan sp = spans[b];
+    mcGradSpan next = spans[numSpans - 1 - blockIdx.x];
+    for (int b = blockIdx.x; b < numSpans; b += gridDim.x) {   // (from the end: what the norm read last is still in the caches)
+        const mcGradSpan sp = next;
+        next = spans[max(numSpans - 1 - b - (int)gridDim.x, 0)];
         if (!sp.out || (sp.out == sp.grad && factor * sp.scale == 1.f)) continue;
         if (factor == 0.f) {   // not a product: the gradients hold what made the norm infinite
             if (sp.outType == MC_F32) span_zero(static_cast<float*>(sp.out), sp.count);
@@ -124,20 +141,33 @@ __global__ void __launch_bounds__(GT) k_weights_update_clipped(float* w, float* 
                                                                int numSpans, const float* __restrict__ normAndFactor) {
     const float f = normAndFactor[1];
     if (f == 0.f) return;   // the norm is not finite: the step is dropped
-    for (int b = blockIdx.x; b < numSpans; b += gridDim.x) {
-        const mcUpdateSpan sp = spans[b];
+    mcUpdateSpan next = spans[numSpans - 1 - blockIdx.x];
+    for (int b = blockIdx.x; b < numSpans; b += gridDim.x) {   // (from the end, as above)
+        const mcUpdateSpan sp = next;
+        next = spans[max(numSpans - 1 - b - (int)gridDim.x, 0)];
         float *W = w + sp.start, *I = inc + sp.start;
         const float* G = grad + sp.start;
-        const unsigned n4 = sp.count / 4;
-        for (unsigned v = threadIdx.x; v < n4; v += GT) {
-            float4 ww = reinterpret_cast<float4*>(W)[v], ii = reinterpret_cast<float4*>(I)[v];
-            const float4 gg = reinterpret_cast<const float4*>(G)[v];
-            step(ww.x, ii.x, gg.x, f, sp.mom, sp.wceps); step(ww.y, ii.y, gg.y, f, sp.mom, sp.wceps);
-            step(ww.z, ii.z, gg.z, f, sp.mom, sp.wceps); step(ww.w, ii.w, gg.w, f, sp.mom, sp.wceps);
-            reinterpret_cast<float4*>(I)[v] = ii;
-            reinterpret_cast<float4*>(W)[v] = ww;
+        constexpr int U = 4;
+        unsigned v = 0;
+        for (; v + GT * 4 * U <= sp.count; v += GT * 4 * U) {
+            Pack<float, 4> ww[U], ii[U], gg[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const unsigned at = v + (u * GT + threadIdx.x) * 4;
+                ww[u] = load_pack<float, 4>(W + at);
+                ii[u] = load_pack<float, 4>(I + at);
+                gg[u] = load_pack<float, 4>(G + at);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const unsigned at = v + (u * GT + threadIdx.x) * 4;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) step(ww[u].v[k], ii[u].v[k], gg[u].v[k], f, sp.mom, sp.wceps);
+                store_pack<float, 4>(I + at, ii[u]);
+                store_pack<float, 4>(W + at, ww[u]);
+            }
         }
-        for (unsigned v = n4 * 4 + threadIdx.x; v < sp.count; v += GT) step(W[v], I[v], G[v], f, sp.mom, sp.wceps);
+        for (v += threadIdx.x; v < sp.count; v += GT) step(W[v], I[v], G[v], f, sp.mom, sp.wceps);
     }
 }
 

@@ -262,17 +262,11 @@ template <class T, int N>
 struct Words {
     static constexpr int COUNT = N * sizeof(T) < 4 ? 1 : N * sizeof(T) / 4;
     unsigned w[COUNT];
-    struct __attribute__((packed, aligned(sizeof(T)), may_alias)) Memory { unsigned w[COUNT]; };
     __device__ __forceinline__ void load(const T* p) {
-        if (N * sizeof(T) < 4) {   // one 16-bit element
-            unsigned short h;
-            __builtin_memcpy(&h, p, 2);
-            w[0] = h;
-            return;
-        }
-        const Memory m = *reinterpret_cast<const Memory*>(p);
-#pragma unroll
-        for (int i = 0; i < COUNT; ++i) w[i] = m.w[i];
+        typedef typename Raw<N * sizeof(T), sizeof(T)>::type R;
+        const R r = __builtin_nontemporal_load(reinterpret_cast<const R*>(p));
+        w[0] = 0;
+        __builtin_memcpy(w, &r, N * sizeof(T));
     }
     __device__ __forceinline__ void fill() {   // -inf
         const unsigned inf = sizeof(T) == 4 ? 0xff800000u : __is_same(T, _Float16) ? 0xfc00fc00u : 0xff80ff80u;
