@@ -12,6 +12,7 @@ namespace mc {
 namespace {
 
 constexpr int GT = 256;             // threads of a workgroup
+constexpr int kSpan = 4096;         // elements of a span, at most
 constexpr int kMaxPartials = 2048;  // workgroups of the first pass = partial sums of the second
 
 __device__ __forceinline__ double block_sum(double v, double* sh) {
@@ -25,44 +26,51 @@ __device__ __forceinline__ double block_sum(double v, double* sh) {
     return r;
 }
 
-template <class T>
-__device__ __forceinline__ void add_square(double& acc, T x) {
-    const double d = (double)(float)x;
-    acc += d * d;
+// The packs of a span, U loads in flight a thread: past the end the last pack is loaded again and not counted.
+template <class T, bool NT>
+__device__ __forceinline__ double span_square(const T* g, unsigned n) {
+    constexpr int V = 16 / sizeof(T), U = 4;
+    const unsigned packs = n / V;
+    double acc = 0.0;
+    for (unsigned at = threadIdx.x; at - threadIdx.x < packs; at += GT * U) {
+        Words<T, V> x[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) x[u].template load<NT>(g + min(at + u * GT, packs - 1) * V);
+        const Pass pass;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            double s = 0.0;
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                const double d = (double)x[u].at(k, pass);
+                s += d * d;
+            }
+            acc += at + u * GT < packs ? s : 0.0;
+            asm volatile("" : "+v"(acc));   // one pack's doubles in registers at a time
+        }
+    }
+    if (threadIdx.x < n - packs * V) {
+        const double d = (double)(float)load_pack<T, 1>(g + packs * V + threadIdx.x, NT).v[0];
+        acc += d * d;
+    }
+    return acc;
 }
 template <class T>
-__device__ __forceinline__ double span_square(const T* g, unsigned n) {
-    constexpr int V = 16 / sizeof(T), U = 8;   // U loads in flight a thread
-    double acc[2] = {0.0, 0.0};
-    unsigned i = 0;
-    for (; i + GT * V * U <= n; i += GT * V * U) {
-        Pack<T, V> x[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) x[u] = load_pack<T, V>(g + i + (u * GT + threadIdx.x) * V);
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int k = 0; k < V; ++k) add_square(acc[k & 1], x[u].v[k]);
-    }
-    for (; i + GT * V <= n; i += GT * V) {
-        const Pack<T, V> x = load_pack<T, V>(g + i + threadIdx.x * V);
-#pragma unroll
-        for (int k = 0; k < V; ++k) add_square(acc[k & 1], x.v[k]);
-    }
-    for (i += threadIdx.x; i < n; i += GT) add_square(acc[0], g[i]);
-    return acc[0] + acc[1];
+__device__ __forceinline__ double span_square(const mcGradSpan& sp, bool nt) {
+    const T* g = static_cast<const T*>(sp.grad);
+    return nt ? span_square<T, true>(g, sp.count) : span_square<T, false>(g, sp.count);
 }
 
-__global__ void __launch_bounds__(GT) k_grad_square(const mcGradSpan* __restrict__ spans, int numSpans, double* __restrict__ partials) {
+__global__ void __launch_bounds__(GT) k_grad_square(const mcGradSpan* __restrict__ spans, int numSpans, double* __restrict__ partials, bool nt) {
     __shared__ double sh[GT / 64];
     double acc = 0.0;
     mcGradSpan sp = spans[blockIdx.x];
     for (int b = blockIdx.x; b < numSpans; b += gridDim.x) {
         const mcGradSpan next = spans[min(b + (int)gridDim.x, numSpans - 1)];   // its way to memory is as long as a gradient's
         double s = 0.0;
-        if (sp.gradType == MC_F32) s = span_square(static_cast<const float*>(sp.grad), sp.count);
-        else if (sp.gradType == MC_F16) s = span_square(static_cast<const _Float16*>(sp.grad), sp.count);
-        else s = span_square(static_cast<const __bf16*>(sp.grad), sp.count);
+        if (sp.gradType == MC_F32) s = span_square<float>(sp, nt);
+        else if (sp.gradType == MC_F16) s = span_square<_Float16>(sp, nt);
+        else s = span_square<__bf16>(sp, nt);
         acc += s * ((double)sp.scale * (double)sp.scale);
         sp = next;
     }
@@ -84,51 +92,42 @@ __global__ void __launch_bounds__(GT) k_grad_factor(const double* __restrict__ p
     }
 }
 
+// One pack of 4 elements a thread: a workgroup takes a quarter of a span.  (Streams of small tiles in the order of memory copy faster than
+// workgroups that walk through stretches of their own: 256 Mi elements bf16 -> float32 in 238 us against 281.)
 template <class T, class O>
-__device__ __forceinline__ void span_scale(const T* g, O* out, unsigned n, float f) {
-    constexpr int V = 16 / (sizeof(T) > sizeof(O) ? sizeof(T) : sizeof(O)), U = 4;
-    unsigned i = 0;
-    for (; i + GT * V * U <= n; i += GT * V * U) {
-        Pack<T, V> x[U];
+__device__ __forceinline__ void tile_scale(const T* g, O* out, unsigned at, unsigned n, float f, bool nt) {
+    if (at + 4 <= n) {
+        const Pack<T, 4> x = load_pack<T, 4>(g + at, nt);
+        Pack<O, 4> y;
 #pragma unroll
-        for (int u = 0; u < U; ++u) x[u] = load_pack<T, V>(g + i + (u * GT + threadIdx.x) * V);
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            Pack<O, V> y;
-#pragma unroll
-            for (int k = 0; k < V; ++k) y.v[k] = (O)((float)x[u].v[k] * f);
-            store_pack<O, V>(out + i + (u * GT + threadIdx.x) * V, y);
+        for (int k = 0; k < 4; ++k) y.v[k] = f == 0.f ? (O)0.f : (O)((float)x.v[k] * f);
+        store_pack<O, 4>(out + at, y, nt);
+    } else
+        for (; at < n; ++at) {
+            const float x = (float)load_pack<T, 1>(g + at, false).v[0];
+            Pack<O, 1> y;
+            y.v[0] = f == 0.f ? (O)0.f : (O)(x * f);
+            store_pack<O, 1>(out + at, y, false);
         }
-    }
-    for (i += threadIdx.x; i < n; i += GT) out[i] = (O)((float)g[i] * f);
-}
-template <class O>
-__device__ __forceinline__ void span_zero(O* out, unsigned n) {
-    for (unsigned i = threadIdx.x; i < n; i += GT) out[i] = (O)0.f;
 }
 template <class T>
-__device__ __forceinline__ void span_clip(const mcGradSpan& sp, float factor) {
+__device__ __forceinline__ void tile_clip(const mcGradSpan& sp, unsigned at, float f, bool nt) {
     const T* g = static_cast<const T*>(sp.grad);
-    const float f = factor * sp.scale;
-    if (sp.outType == MC_F32) span_scale(g, static_cast<float*>(sp.out), sp.count, f);
-    else if (sp.outType == MC_F16) span_scale(g, static_cast<_Float16*>(sp.out), sp.count, f);
-    else span_scale(g, static_cast<__bf16*>(sp.out), sp.count, f);
+    if (sp.outType == MC_F32) tile_scale(g, static_cast<float*>(sp.out), at, sp.count, f, nt);
+    else if (sp.outType == MC_F16) tile_scale(g, static_cast<_Float16*>(sp.out), at, sp.count, f, nt);
+    else tile_scale(g, static_cast<__bf16*>(sp.out), at, sp.count, f, nt);
 }
 
-__global__ void __launch_bounds__(GT) k_clip_grads(const mcGradSpan* __restrict__ spans, int numSpans, const float* __restrict__ normAndFactor) {
-    const float factor = normAndFactor[1];
-    mcGradSpan next = spans[numSpans - 1 - blockIdx.x];
-    for (int b = blockIdx.x; b < numSpans; b += gridDim.x) {   // (from the end: what the norm read last is still in the caches)
-        const mcGradSpan sp = next;
-        next = spans[max(numSpans - 1 - b - (int)gridDim.x, 0)];
-        if (!sp.out || (sp.out == sp.grad && factor * sp.scale == 1.f)) continue;
-        if (factor == 0.f) {   // not a product: the gradients hold what made the norm infinite
-            if (sp.outType == MC_F32) span_zero(static_cast<float*>(sp.out), sp.count);
-            else span_zero(static_cast<_Float16*>(sp.out), sp.count);
-        } else if (sp.gradType == MC_F32) span_clip<float>(sp, factor);
-        else if (sp.gradType == MC_F16) span_clip<_Float16>(sp, factor);
-        else span_clip<__bf16>(sp, factor);
-    }
+// Factor 0 writes zeros and not products: the gradients hold what made the norm infinite.
+__global__ void __launch_bounds__(GT) k_clip_grads(const mcGradSpan* __restrict__ spans, const float* __restrict__ normAndFactor, bool nt) {
+    const mcGradSpan sp = spans[blockIdx.x / (kSpan / (GT * 4))];
+    const unsigned at = (blockIdx.x % (kSpan / (GT * 4)) * GT + threadIdx.x) * 4;
+    if (at >= sp.count || !sp.out) return;
+    const float f = normAndFactor[1] == 0.f ? 0.f : normAndFactor[1] * sp.scale;
+    if (sp.out == sp.grad && f == 1.f) return;
+    if (sp.gradType == MC_F32) tile_clip<float>(sp, at, f, nt);
+    else if (sp.gradType == MC_F16) tile_clip<_Float16>(sp, at, f, nt);
+    else tile_clip<__bf16>(sp, at, f, nt);
 }
 
 // inc = mom*inc + factor*grad; inc += wceps*W; W += inc, in the order (and, at factor 1, with the bits) of mc_weights_update_spans.
@@ -137,38 +136,44 @@ __device__ __forceinline__ void step(float& w, float& i, float g, float f, float
     if (wceps != 0.f) i = fmaf(wceps, w, i);
     w += i;
 }
+// A workgroup takes a span, with up to 12 loads in flight a thread.
 __global__ void __launch_bounds__(GT) k_weights_update_clipped(float* w, float* inc, const float* __restrict__ grad, const mcUpdateSpan* __restrict__ spans,
-                                                               int numSpans, const float* __restrict__ normAndFactor) {
+                                                               const float* __restrict__ normAndFactor, bool nt) {
+    const mcUpdateSpan sp = spans[blockIdx.x];
     const float f = normAndFactor[1];
     if (f == 0.f) return;   // the norm is not finite: the step is dropped
-    mcUpdateSpan next = spans[numSpans - 1 - blockIdx.x];
-    for (int b = blockIdx.x; b < numSpans; b += gridDim.x) {   // (from the end, as above)
-        const mcUpdateSpan sp = next;
-        next = spans[max(numSpans - 1 - b - (int)gridDim.x, 0)];
-        float *W = w + sp.start, *I = inc + sp.start;
-        const float* G = grad + sp.start;
-        constexpr int U = 4;
-        unsigned v = 0;
-        for (; v + GT * 4 * U <= sp.count; v += GT * 4 * U) {
-            Pack<float, 4> ww[U], ii[U], gg[U];
+    float *W = w + sp.start, *I = inc + sp.start;
+    const float* G = grad + sp.start;
+    constexpr int U = 4;
+    unsigned v = 0;
+    for (; v + GT * 4 * U <= sp.count; v += GT * 4 * U) {
+        Pack<float, 4> ww[U], ii[U], gg[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const unsigned at = v + (u * GT + threadIdx.x) * 4;
-                ww[u] = load_pack<float, 4>(W + at);
-                ii[u] = load_pack<float, 4>(I + at);
-                gg[u] = load_pack<float, 4>(G + at);
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const unsigned at = v + (u * GT + threadIdx.x) * 4;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) step(ww[u].v[k], ii[u].v[k], gg[u].v[k], f, sp.mom, sp.wceps);
-                store_pack<float, 4>(I + at, ii[u]);
-                store_pack<float, 4>(W + at, ww[u]);
-            }
+        for (int u = 0; u < U; ++u) {
+            const unsigned at = v + (u * GT + threadIdx.x) * 4;
+            ww[u] = load_pack<float, 4>(W + at, nt);
+            ii[u] = load_pack<float, 4>(I + at, nt);
+            gg[u] = load_pack<float, 4>(G + at, nt);
         }
-        for (v += threadIdx.x; v < sp.count; v += GT) step(W[v], I[v], G[v], f, sp.mom, sp.wceps);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const unsigned at = v + (u * GT + threadIdx.x) * 4;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) step(ww[u].v[k], ii[u].v[k], gg[u].v[k], f, sp.mom, sp.wceps);
+            store_pack<float, 4>(I + at, ii[u], nt);
+            store_pack<float, 4>(W + at, ww[u], nt);
+        }
     }
+    const unsigned end = sp.count / 4 * 4;
+    for (v += threadIdx.x * 4; v < end; v += GT * 4) {
+        Pack<float, 4> ww = load_pack<float, 4>(W + v, nt), ii = load_pack<float, 4>(I + v, nt);
+        const Pack<float, 4> gg = load_pack<float, 4>(G + v, nt);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) step(ww.v[k], ii.v[k], gg.v[k], f, sp.mom, sp.wceps);
+        store_pack<float, 4>(I + v, ii, nt);
+        store_pack<float, 4>(W + v, ww, nt);
+    }
+    if (end + threadIdx.x < sp.count) step(W[end + threadIdx.x], I[end + threadIdx.x], G[end + threadIdx.x], f, sp.mom, sp.wceps);
 }
 
 int partials_for(int numSpans) { return std::max(1, std::min(numSpans, kMaxPartials)); }
@@ -197,7 +202,6 @@ int mc_grad_spans(const mcGradTensor* tensors, int numTensors, mcGradSpan* spans
     MC_REQUIRE(numSpans && numTensors >= 0 && (tensors || numTensors == 0), "mc_grad_spans: bad arguments");
     *numSpans = 0;
     try {
-        unsigned long long total = 0;
         std::vector<Range> ranges;
         for (int i = 0; i < numTensors; ++i) {
             const mcGradTensor& t = tensors[i];
@@ -211,39 +215,39 @@ int mc_grad_spans(const mcGradTensor* tensors, int numTensors, mcGradSpan* spans
             MC_REQUIRE(t.out != t.grad || t.gradType == t.outType, "mc_grad_spans: tensor %d: in place needs one element type", i);
             ranges.push_back({(size_t)t.grad, (size_t)t.grad + t.count * gs, t.out == t.grad});
             if (t.out && t.out != t.grad) ranges.push_back({(size_t)t.out, (size_t)t.out + t.count * os, true});
-            total += t.count;
         }
         MC_REQUIRE(!ranges_clash(ranges), "mc_grad_spans: an output overlaps another output or gradient");
-        // Spans of a power of two elements: at least 4096 (a span's descriptor and its workgroup cost then less than its bytes), and about
-        // 8192 spans in all, four rounds of the first pass's workgroups, so that a large list's last round is short.
-        unsigned long long per = 4096;
-        while (per < 65536 && per * 8192 < total) per *= 2;
+        // Spans of kSpan elements, cut so that all but a tensor's first begin on a 128-byte line of what is written (of what is read, where
+        // nothing is): lines that two workgroups write in halves cost a fifth of the copy's time.
         unsigned long long n = 0;
-        for (int i = 0; i < numTensors; ++i) n += (tensors[i].count + per - 1) / per;
-        MC_REQUIRE(n <= 0x7fffffffull, "mc_grad_spans: too many elements");
-        *numSpans = (int)n;
-        if (!spans) return MC_OK;
-        MC_REQUIRE((unsigned long long)std::max(maxSpans, 0) >= n, "mc_grad_spans: %llu spans, room for %d", n, maxSpans);
-        int at = 0;
         for (int i = 0; i < numTensors; ++i) {
             const mcGradTensor& t = tensors[i];
-            for (unsigned long long done = 0; done < t.count; done += per) {
+            for (unsigned long long done = 0; done < t.count;) {
                 mcGradSpan sp;
                 sp.grad = static_cast<const char*>(t.grad) + done * elem_size(t.gradType);
                 sp.out = t.out ? static_cast<char*>(t.out) + done * elem_size(t.outType) : nullptr;
-                sp.count = (unsigned)std::min(per, t.count - done);
+                const unsigned past = sp.out ? (size_t)sp.out % 128 / elem_size(t.outType) : (size_t)sp.grad % 128 / elem_size(t.gradType);
+                sp.count = (unsigned)std::min<unsigned long long>(kSpan - past, t.count - done);
                 sp.scale = t.scale;
                 sp.gradType = t.gradType;
                 sp.outType = t.outType;
-                spans[at++] = sp;
+                if (spans && n < (unsigned long long)std::max(maxSpans, 0)) spans[n] = sp;
+                ++n;
+                done += sp.count;
             }
+            MC_REQUIRE(n <= 0x1fffffffull, "mc_grad_spans: too many elements");
         }
+        *numSpans = (int)n;
+        MC_REQUIRE(!spans || (unsigned long long)std::max(maxSpans, 0) >= n, "mc_grad_spans: %llu spans, room for %d", n, maxSpans);
     } catch (const std::exception& e) {
         set_error("mc_grad_spans: %s", e.what());
         return MC_EINVAL;
     }
     return MC_OK;
 }
+
+// Spans are nearly all of kSpan elements where there are so many that streaming pays.
+static bool spans_stream(int numSpans) { return streams((size_t)numSpans * kSpan * 2); }
 
 size_t mc_grad_norm_workspace_bytes(int numSpans) { return (size_t)partials_for(numSpans) * sizeof(double); }
 
@@ -258,7 +262,7 @@ int mc_grad_norm(const mcGradSpan* spansDevice, int numSpans, float maxNorm, flo
     }
     double* partials = static_cast<double*>(workspace);
     const int n = numSpans ? partials_for(numSpans) : 0;
-    if (n) hipLaunchKernelGGL(k_grad_square, dim3(n), dim3(GT), 0, S(s), spansDevice, numSpans, partials);
+    if (n) hipLaunchKernelGGL(k_grad_square, dim3(n), dim3(GT), 0, S(s), spansDevice, numSpans, partials, spans_stream(numSpans));
     hipLaunchKernelGGL(k_grad_factor, dim3(1), dim3(GT), 0, S(s), partials, n, maxNorm, normAndFactor);
     return launch_status("mc_grad_norm");
 }
@@ -267,7 +271,8 @@ int mc_clip_grads(const mcGradSpan* spansDevice, int numSpans, const float* norm
     MC_REQUIRE(normAndFactor && numSpans >= 0 && (spansDevice || numSpans == 0), "mc_clip_grads: bad arguments");
     MC_REQUIRE(stream_on_current_device(s), "mc_clip_grads: the stream belongs to another device than the current one");
     if (numSpans == 0) return MC_OK;
-    hipLaunchKernelGGL(k_clip_grads, dim3(std::min(numSpans, 8 * num_cus())), dim3(GT), 0, S(s), spansDevice, numSpans, normAndFactor);
+    MC_REQUIRE(numSpans <= 0x1fffffff, "mc_clip_grads: too many spans");
+    hipLaunchKernelGGL(k_clip_grads, dim3(numSpans * (kSpan / (GT * 4))), dim3(GT), 0, S(s), spansDevice, normAndFactor, spans_stream(numSpans));
     return launch_status("mc_clip_grads");
 }
 
@@ -277,8 +282,8 @@ int mc_weights_update_spans_clipped(float* weights, float* inc, const float* gra
     MC_REQUIRE(aligned16(weights) && aligned16(inc) && aligned16(grad), "mc_weights_update_spans_clipped: arenas must be 16-byte aligned");
     MC_REQUIRE(stream_on_current_device(s), "mc_weights_update_spans_clipped: the stream belongs to another device than the current one");
     if (numSpans <= 0) return MC_OK;
-    hipLaunchKernelGGL(k_weights_update_clipped, dim3(std::min(numSpans, 8 * num_cus())), dim3(GT), 0, S(s), weights, inc, grad, spansDevice, numSpans,
-                       normAndFactor);
+    hipLaunchKernelGGL(k_weights_update_clipped, dim3(numSpans), dim3(GT), 0, S(s), weights, inc, grad, spansDevice, normAndFactor,
+                       spans_stream(numSpans));
     return launch_status("mc_weights_update_spans_clipped");
 }
 

@@ -23,6 +23,7 @@ struct LogProbArgs {
     int* topClasses;
     float* topLogProbs;
     int numTop;
+    bool nt;                      // the logits are read past the caches
 };
 
 // What a workgroup leaves of its classes of a case for the joining kernel; its best numTop keys follow in an array of their own.
@@ -108,43 +109,38 @@ __device__ __forceinline__ int key_class(unsigned long long key) { return (int)(
 
 constexpr int kCand = 256;   // candidates a group's list holds
 
-// A value that at least k of the group's maxima (one in each of `values`, over `lanes` neighbouring lanes of a wave) reach and few more
-// do: at least k classes reach it then, so no class below it is among the best k.  Bisection between the least finite maximum and
-// the largest; where ties or the step limit stop it early the value is lower than it could be, never too high.
+// A value that at least k of the group's maxima (v, Q in each of the wave's lanes that `mask` names, the largest of them hi) reach and
+// few more do: at least k classes reach it then, so no class below it is among the best k.  First down from hi in growing steps, then
+// by bisection; ballots count.  Where ties or the step limits stop it early the value is lower than it could be, never too high.
 template <int Q>
-__device__ __forceinline__ float top_threshold(const float (&v)[Q], int k, int lanes) {
-    float lo = INFINITY, hi = -INFINITY;
-    int finite = 0;
-#pragma unroll
-    for (int q = 0; q < Q; ++q)
-        if (v[q] > -INFINITY) {
-            lo = fminf(lo, v[q]);
-            hi = fmaxf(hi, v[q]);
-            ++finite;
-        }
-    for (int off = lanes / 2; off > 0; off >>= 1) {
-        lo = fminf(lo, __shfl_xor(lo, off, 64));
-        hi = fmaxf(hi, __shfl_xor(hi, off, 64));
-        finite += __shfl_xor(finite, off, 64);
-    }
-    if (finite <= k) return -INFINITY;
-    const int enough = k + k / 4 + 1;
-    int reached = finite;
-    for (int it = 0; it < 24 && __any(reached > enough); ++it) {   // (lanes of other cases may still be at it)
-        const float mid = 0.5f * lo + 0.5f * hi;
+__device__ __forceinline__ float top_threshold(const float (&v)[Q], int k, float hi, unsigned long long mask) {
+    const auto reach = [&](float y) {
         int count = 0;
 #pragma unroll
-        for (int q = 0; q < Q; ++q) count += v[q] >= mid;
-        for (int off = lanes / 2; off > 0; off >>= 1) count += __shfl_xor(count, off, 64);
-        if (reached > enough) {
-            if (count >= k) {
-                lo = mid;
-                reached = count;
-            } else hi = mid;
-        }
+        for (int q = 0; q < Q; ++q) count += __popcll(__ballot(v[q] >= y) & mask);
+        return count;
+    };
+    if (!(hi > -INFINITY)) return -INFINITY;
+    float lo = hi, above = hi, step = fmaxf(1.f, fabsf(hi) * 0x1p-18f);
+    int reached = reach(lo);
+    for (int it = 0; it < 24 && reached < k; ++it, step *= 4.f) {
+        above = lo;
+        lo = hi - step;
+        reached = reach(lo);
+    }
+    if (reached < k) return -INFINITY;
+    const int enough = k + k / 4 + 1;
+    for (int it = 0; it < 24 && reached > enough; ++it) {
+        const float mid = 0.5f * lo + 0.5f * above;
+        const int count = reach(mid);
+        if (count >= k) {
+            lo = mid;
+            reached = count;
+        } else above = mid;
     }
     return lo;
 }
+constexpr int kFewClasses = 64;   // so many can all be candidates: ordering them costs less than finding a threshold
 
 // The k largest keys of classes [from, to) in one walk over them in order: THREADS classes at a time against the k-th best so far;
 // what beats it joins the list, which is ordered again by counting, for each key, the larger ones.  Any number of ties, any order; used
@@ -244,79 +240,65 @@ __device__ __forceinline__ void take_back(float m, float& s, float& w) {
     w = (w - d * s) * f;
     s *= f;
 }
-// s and w of x(0) ... x(COUNT - 1).  A t of -inf is a ruled-out class: its 2^t is 0 and so has to be its t 2^t.
+// s and w of t(0) ... t(COUNT - 1).  A ruled-out class has t = -inf and 2^t = 0, and so has to have t 2^t; without that guard w is NaN where
+// there is one, and guarded() forms it again.
 template <bool ENT, int COUNT, class F>
-__device__ __forceinline__ void sums_of(F x, Shift h, float& s, float& w) {
+__device__ __forceinline__ void sums_of(F t, float& s, float& w) {
     s = w = 0.f;
 #pragma unroll
     for (int i = 0; i < COUNT; ++i) {
-        const float t = fmaf(x(i), h.scale, -h.c), e = __builtin_amdgcn_exp2f(t);
+        const float x = t(i), e = __builtin_amdgcn_exp2f(x);
         s += e;
-        if (ENT) w = fmaf(e, fmaxf(t, -200.f), w);
+        if (ENT) w = fmaf(e, x, w);
     }
+    asm volatile("" : "+v"(s));   // here, and not with every e kept until s is used
+}
+template <int COUNT, class F>
+__device__ __forceinline__ float guarded(F t) {
+    float w = 0.f;
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) {
+        const float x = t(i);
+        w = fmaf(__builtin_amdgcn_exp2f(x), fmaxf(x, -200.f), w);
+    }
+    return w;
 }
 
-// N elements of type T as the registers they were loaded into.  Elements are converted where they are used; keep() stops the compiler
-// from holding the converted values from one use to the next, which would take twice the registers for 16-bit types.
+// The largest element of a pack.
 template <class T, int N>
-struct Words {
-    static constexpr int COUNT = N * sizeof(T) < 4 ? 1 : N * sizeof(T) / 4;
-    unsigned w[COUNT];
-    __device__ __forceinline__ void load(const T* p) {
-        typedef typename Raw<N * sizeof(T), sizeof(T)>::type R;
-        const R r = __builtin_nontemporal_load(reinterpret_cast<const R*>(p));
-        w[0] = 0;
-        __builtin_memcpy(w, &r, N * sizeof(T));
-    }
-    __device__ __forceinline__ void fill() {   // -inf
-        const unsigned inf = sizeof(T) == 4 ? 0xff800000u : __is_same(T, _Float16) ? 0xfc00fc00u : 0xff80ff80u;
+__device__ __forceinline__ float max_in(const Words<T, N>& v, Pass p) {
+    if (!__is_same(T, _Float16) || N == 1) return max_of<N>([&](int k) { return v.at(k, p); });
+    Words<T, 2> m;   // two at a time
+    m.w[0] = v.w[0];
 #pragma unroll
-        for (int i = 0; i < COUNT; ++i) w[i] = inf;
-    }
-    __device__ __forceinline__ void fill_first(int n) {   // -inf in the first n of them
-        const unsigned inf = sizeof(T) == 4 ? 0xff800000u : __is_same(T, _Float16) ? 0xfc00fc00u : 0xff80ff80u;
-        constexpr int PER = sizeof(T) == 4 ? 1 : 2;
-#pragma unroll
-        for (int i = 0; i < COUNT; ++i) {
-            if (PER == 2 && n == 2 * i + 1) w[i] = (w[i] & 0xffff0000u) | (inf & 0xffffu);
-            if (n >= PER * (i + 1)) w[i] = inf;
-        }
-    }
-    __device__ __forceinline__ void set(int k, T v) {
-        unsigned short h = 0;
-        if (sizeof(T) == 4) {
-            __builtin_memcpy(&w[k], &v, sizeof(T));
-            return;
-        }
-        __builtin_memcpy(&h, &v, 2);
-        w[k / 2] = k % 2 ? (w[k / 2] & 0xffffu) | (unsigned)h << 16 : (w[k / 2] & 0xffff0000u) | h;
-    }
-    __device__ __forceinline__ float at(int k) const {
-        if (sizeof(T) == 4) return __uint_as_float(w[k]);
-        const unsigned u = w[k / 2];
-        if (__is_same(T, __bf16)) return __uint_as_float(k % 2 ? u & 0xffff0000u : u << 16);
-        const unsigned short h = (unsigned short)(k % 2 ? u >> 16 : u);
-        _Float16 v;
-        __builtin_memcpy(&v, &h, 2);
-        return (float)v;
-    }
-    __device__ __forceinline__ void keep() {
-#pragma unroll
-        for (int i = 0; i < COUNT; ++i) asm("" : "+v"(w[i]));
-    }
-};
+    for (int i = 1; i < v.COUNT; ++i) asm("v_pk_max_f16 %0, %1, %2" : "=v"(m.w[0]) : "v"(m.w[0]), "v"(v.w[i]));
+    return fmaxf(m.at(0, p), m.at(1, p));
+}
+// Element k as fma(x, scale, -c); a half goes into the fma as it is (volatile: see Pass).
+template <class T, int N>
+__device__ __forceinline__ float shifted(const Words<T, N>& v, int k, Shift h, Pass p) {
+    if (!__is_same(T, _Float16)) return fmaf(v.at(k, p), h.scale, -h.c);
+    float t;
+    if (k % 2) asm volatile("v_fma_mix_f32 %0, %1, %2, -%3 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(t) : "v"(v.w[k / 2]), "v"(h.scale), "v"(h.c));
+    else asm volatile("v_fma_mix_f32 %0, %1, %2, -%3 op_sel:[0,0,0] op_sel_hi:[1,0,0]" : "=v"(t) : "v"(v.w[k / 2]), "v"(h.scale), "v"(h.c));
+    return t;
+}
 
 // ---------------------------------------------------------------- a case's classes side by side
 // A workgroup (or wave) takes up to THREADS * U packs of 16 bytes of one case into registers in one burst of loads, and does all the
 // rest there: the largest logit, the sums against it, the candidates for the top.
+constexpr int kPacks = 128;
 template <class T, int THREADS, int U, bool ENT, bool TOP>
-__global__ void __launch_bounds__(LT) k_log_probs_rows(LogProbArgs a, Parts p) {
+__global__ void __launch_bounds__(LT) __attribute__((amdgpu_waves_per_eu(4))) k_log_probs_rows(LogProbArgs a, Parts p) {
     typedef Group<THREADS> G;
     constexpr int V = 16 / sizeof(T), GROUPS = LT / THREADS;
     __shared__ float shRed[GROUPS][3 * (G::WAVES > 1 ? G::WAVES : 1)];
     __shared__ float shMax[TOP ? LT : 1];
     __shared__ unsigned long long shCand[TOP ? GROUPS : 1][TOP ? kCand + MC_MAX_TOP : 1];
-    __shared__ int shCount[GROUPS];
+    // the packs that hold candidates, and where they are from
+    constexpr int PACKS = kPacks / GROUPS;
+    __shared__ unsigned shPack[TOP ? GROUPS : 1][TOP ? PACKS : 1][4], shFrom[TOP ? GROUPS : 1][TOP ? PACKS : 1];
+    __shared__ int shPacks[GROUPS], shCount[GROUPS];
     const int group = G::index(), tid = G::tid();
     const unsigned item = blockIdx.x * GROUPS + group, row = item / (unsigned)p.parts;
     if (row >= (unsigned)a.numCases) return;          // (whole waves: THREADS is 64 then)
@@ -333,8 +315,13 @@ __global__ void __launch_bounds__(LT) k_log_probs_rows(LogProbArgs a, Parts p) {
     const bool whole = THREADS == LT || a.numOut >= V;
     if (whole) {
         const T* from = x - back;
+        if (a.nt) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) v[u].load(from + (unsigned)(min(first + u * (THREADS * V), last) + back));
+            for (int u = 0; u < U; ++u) v[u].template load<true>(from + (unsigned)(min(first + u * (THREADS * V), last) + back));
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; ++u) v[u].template load<false>(from + (unsigned)(min(first + u * (THREADS * V), last) + back));
+        }
         if (len != THREADS * U * V) {
 #pragma unroll
             for (int u = 0; u < U; ++u) v[u].fill_first(first + u * (THREADS * V) - last);
@@ -349,19 +336,29 @@ __global__ void __launch_bounds__(LT) k_log_probs_rows(LogProbArgs a, Parts p) {
     const float labelLogit = label >= 0 ? (float)x[label] : 0.f;   // (one part: lo is 0)
 
     float pm[U];
+    {
+        const Pass pass;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        pm[u] = max_of<V>([&](int k) { return v[u].at(k); });
-        v[u].keep();
+        for (int u = 0; u < U; ++u) pm[u] = max_in(v[u], pass);
     }
     const float mine = max_of<U>([&](int u) { return pm[u]; });
     if (TOP) {
         shMax[threadIdx.x] = mine;
-        if (tid == 0) shCount[group] = 0;
+        if (tid == 0) shCount[group] = shPacks[group] = 0;
     }
     const float m = G::max(mine, shRed[group]);
     float s, w;
-    sums_of<ENT, U * V>([&](int i) { return v[i / V].at(i % V); }, shift_for(m), s, w);
+    const Shift h = shift_for(m);
+    {
+        const Pass pass;
+        sums_of<ENT, U * V>([&](int i) { return shifted(v[i / V], i % V, h, pass); }, s, w);
+    }
+    if (ENT && __any(w != w)) {   // ruled-out classes (or NaN): again, with the guard that the usual case is spared
+        Shift again = h;
+        asm volatile("" : "+v"(again.c));   // (not the values of before, kept)
+        const Pass pass;
+        w = guarded<U * V>([&](int i) { return fmaf(v[i / V].at(i % V, pass), again.scale, -again.c); });
+    }
     G::sum2(s, w, shRed[group] + G::WAVES);
     take_back(m, s, w);
     const CaseStats c = case_stats(m, s);
@@ -375,28 +372,37 @@ __global__ void __launch_bounds__(LT) k_log_probs_rows(LogProbArgs a, Parts p) {
     float q[THREADS / 64];
 #pragma unroll
     for (int i = 0; i < THREADS / 64; ++i) q[i] = shMax[group * THREADS + i * 64 + (threadIdx.x & 63)];
-    const float threshold = top_threshold(q, a.numTop, 64);
+    const float threshold = len <= kFewClasses ? -INFINITY : top_threshold(q, a.numTop, m, ~0ull);
 #pragma unroll
     for (int u = 0; u < U; ++u)
-        if (pm[u] >= threshold) {
-            v[u].keep();
+        if (pm[u] >= threshold && pm[u] > -INFINITY) {
+            const int to = atomicAdd(&shPacks[group], 1);
+            if (to < PACKS) {
 #pragma unroll
-            for (int k = 0; k < V; ++k) {
-                const float y = v[u].at(k);
-                if (y >= threshold && y > -INFINITY) {
-                    const int to = atomicAdd(&shCount[group], 1);
-                    if (to < kCand) shCand[group][to] = top_key(y, lo + (whole ? min(first + u * (THREADS * V), last) : 0) + k);
-                }
+                for (int i = 0; i < 4; ++i) shPack[group][to][i] = v[u].w[i];
+                shFrom[group][to] = lo + (whole ? min(first + u * (THREADS * V), last) : 0);
             }
         }
+    G::sync();
+    const int packs = shPacks[group];
+    for (int i = tid; i < min(packs, PACKS) * V; i += THREADS) {   // an element a thread
+        const unsigned word = shPack[group][i / V][i % V * sizeof(T) / 4];
+        Words<T, 4 / sizeof(T)> pair;
+        pair.w[0] = word;
+        const float y = sizeof(T) == 4 || i % 2 == 0 ? pair.at(0, Pass()) : pair.at(sizeof(T) == 4 ? 0 : 1, Pass());
+        if (y >= threshold && y > -INFINITY) {
+            const int to = atomicAdd(&shCount[group], 1);
+            if (to < kCand) shCand[group][to] = top_key(y, shFrom[group][i / V] + i % V);
+        }
+    }
     G::sync();
     const int count = shCount[group];
     const auto put = [&](int rank, unsigned long long key) {
         if (p.parts == 1) write_top(a, n, rank, key, c);
         else p.keys[(size_t)item * a.numTop + rank] = key;
     };
-    if (count <= kCand) rank_keys(shCand[group], count, a.numTop, tid, THREADS, put);
-    else {
+    if (packs <= PACKS && count <= kCand) rank_keys(shCand[group], count, a.numTop, tid, THREADS, put);
+    else {   // ties, or orders that put many of the largest into few packs' reach
         G::sync();
         top_by_scan<THREADS>(x - lo, 1, lo, lo + len, a.numTop, shCand[group] + kCand, shCand[group]);
         if (tid < a.numTop) put(tid, shCand[group][kCand + tid]);
@@ -428,9 +434,12 @@ __global__ void __launch_bounds__(LT) k_log_probs_cols(LogProbArgs a, Parts p, i
     const T* x = static_cast<const T*>(a.logits) + (size_t)n0 * (P == 1 ? a.caseStride : 1);
 
     Words<T, P> v[U];
+    if (a.nt) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        v[u].load(x + (size_t)min(lo + u * R + r, hi - 1) * a.classStride);
+        for (int u = 0; u < U; ++u) v[u].template load<true>(x + (size_t)min(lo + u * R + r, hi - 1) * a.classStride);
+    } else {
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u].template load<false>(x + (size_t)min(lo + u * R + r, hi - 1) * a.classStride);
     }
     if (hi - lo != U * R) {
 #pragma unroll
@@ -438,18 +447,17 @@ __global__ void __launch_bounds__(LT) k_log_probs_cols(LogProbArgs a, Parts p, i
             if (lo + u * R + r >= hi) v[u].fill();
     }
     float pm[TOP ? WINDOWS : 1][P], m[P], s[P], w[P];
+    const Pass first;
 #pragma unroll
     for (int k = 0; k < P; ++k) {
         m[k] = -INFINITY;
 #pragma unroll
         for (int i = 0; i < WINDOWS; ++i) {
-            const float y = max_of<W>([&](int u) { return v[i * W + u].at(k); });
+            const float y = max_of<W>([&](int u) { return v[i * W + u].at(k, first); });
             if (TOP) pm[i][k] = y;
             m[k] = fmaxf(m[k], y);
         }
     }
-#pragma unroll
-    for (int u = 0; u < U; ++u) v[u].keep();
     // TOP: the maxima of WINDOWS * R stretches for each case, [case][stretch]
     float* shSeg = reinterpret_cast<float*>(shDyn + col_list_keys(cases));
     int* shCount = reinterpret_cast<int*>(shSeg + cases * (WINDOWS * R + 1));
@@ -467,10 +475,18 @@ __global__ void __launch_bounds__(LT) k_log_probs_cols(LogProbArgs a, Parts p, i
         if (lane < G) shM[wave][g * P + k] = m[k];
     }
     __syncthreads();
+    const Pass second;
 #pragma unroll
     for (int k = 0; k < P; ++k) {
         m[k] = fmaxf(fmaxf(shM[0][g * P + k], shM[1][g * P + k]), fmaxf(shM[2][g * P + k], shM[3][g * P + k]));
-        sums_of<ENT, U>([&](int i) { return v[i].at(k); }, shift_for(m[k]), s[k], w[k]);
+        const Shift h = shift_for(m[k]);
+        sums_of<ENT, U>([&](int i) { return shifted(v[i], k, h, second); }, s[k], w[k]);
+        if (ENT && __any(w[k] != w[k])) {   // (see the rows)
+            Shift again = h;
+            asm volatile("" : "+v"(again.c));
+            const Pass pass;
+            w[k] = guarded<U>([&](int i) { return fmaf(v[i].at(k, pass), again.scale, -again.c); });
+        }
         for (int off = 32; off >= G; off >>= 1) {
             s[k] += __shfl_xor(s[k], off, 64);
             if (ENT) w[k] += __shfl_xor(w[k], off, 64);
@@ -492,15 +508,13 @@ __global__ void __launch_bounds__(LT) k_log_probs_cols(LogProbArgs a, Parts p, i
             const float labelLogit = label >= 0 ? (float)static_cast<const T*>(a.logits)[(size_t)label * a.classStride + (size_t)n * a.caseStride] : 0.f;
             write_case(a, n, c, S, Wt, label, labelLogit);
             if (TOP) {
-                shS[0][cc] = c.logSum;   // (read by its own thread only until the next barrier)
-                shM[0][cc] = c.m;
+                shS[0][cc] = c.logSum;   // (these two are read by their own thread only until the next barrier)
+                shW[0][cc] = c.m;
             }
         } else p.stats[(size_t)n * p.parts + part] = {M, S, Wt, 0.f};
     }
     if (!TOP) return;
 
-#pragma unroll
-    for (int u = 0; u < U; ++u) v[u].keep();
     // thresholds: `lanes` neighbouring lanes share a case's maxima
     const int lanes = min(64, LT / cases), owner = threadIdx.x / lanes, sub = threadIdx.x % lanes, stretches = WINDOWS * R;
     {
@@ -510,10 +524,14 @@ __global__ void __launch_bounds__(LT) k_log_probs_cols(LogProbArgs a, Parts p, i
             const int at = sub + i * lanes;
             q[i] = owner < cases && at < stretches ? shSeg[owner * (stretches + 1) + at] : -INFINITY;
         }
-        const float tau = top_threshold(q, a.numTop, lanes);
+        const unsigned long long mask = (lanes == 64 ? ~0ull : (1ull << lanes) - 1) << (lane - lane % lanes);
+        const int mine = min(owner, cases - 1);
+        const float most = fmaxf(fmaxf(shM[0][mine], shM[1][mine]), fmaxf(shM[2][mine], shM[3][mine]));
+        const float tau = hi - lo <= kFewClasses / 2 ? -INFINITY : top_threshold(q, a.numTop, most, mask);
         if (owner < cases && sub == 0) shTau[owner] = tau;
     }
     __syncthreads();
+    const Pass third;
 #pragma unroll
     for (int k = 0; k < P; ++k) {
         const float tau = shTau[g * P + k];
@@ -522,7 +540,7 @@ __global__ void __launch_bounds__(LT) k_log_probs_cols(LogProbArgs a, Parts p, i
             if (pm[i][k] >= tau) {
 #pragma unroll
                 for (int u = 0; u < W; ++u) {
-                    const float y = v[i * W + u].at(k);
+                    const float y = v[i * W + u].at(k, third);
                     if (y >= tau && y > -INFINITY) {
                         const int to = atomicAdd(&shCount[g * P + k], 1);
                         if (to < kColCand) shDyn[(g * P + k) * kColCand + to] = top_key(y, lo + (i * W + u) * R + r);
@@ -533,7 +551,7 @@ __global__ void __launch_bounds__(LT) k_log_probs_cols(LogProbArgs a, Parts p, i
     __syncthreads();
     const auto put = [&](int cc, int rank, unsigned long long key) {
         const int n = min((tile * G + cc / P) * P, a.numCases - P) + cc % P;
-        if (p.parts == 1) write_top(a, n, rank, key, CaseStats{shM[0][cc], shS[0][cc], 0.f});
+        if (p.parts == 1) write_top(a, n, rank, key, CaseStats{shW[0][cc], shS[0][cc], 0.f});
         else p.keys[((size_t)n * p.parts + part) * a.numTop + rank] = key;
     };
     if (owner < cases && shCount[owner] <= kColCand)
@@ -583,7 +601,7 @@ __global__ void __launch_bounds__(LT) k_log_probs_join(LogProbArgs a, Parts p) {
     // candidates: keys that reach a value that numTop parts' best keys reach
     const unsigned long long* keys = p.keys + row * p.parts * a.numTop;
     float threshold = -INFINITY;
-    if (p.parts > a.numTop) {
+    if (p.parts > a.numTop && p.parts * a.numTop > kFewClasses) {
         constexpr int Q = 8;
         float q[Q];
         const int parts = min(p.parts, 64 * Q);   // (beyond: the first ones' threshold holds too)
@@ -593,7 +611,7 @@ __global__ void __launch_bounds__(LT) k_log_probs_join(LogProbArgs a, Parts p) {
             const unsigned long long key = at < parts ? keys[(size_t)at * a.numTop] : 0;
             q[i] = key ? key_logit(key) : -INFINITY;
         }
-        threshold = top_threshold(q, a.numTop, 64);
+        threshold = top_threshold(q, a.numTop, m, ~0ull);
     }
     const int total = p.parts * a.numTop;
     G::sync();
@@ -642,6 +660,7 @@ struct LogProbGradArgs {
     void* target;
     size_t targetClassStride, targetCaseStride;
     int add;
+    bool nt;
 };
 
 // d_j = p_j (A - h (ln p_j + H)) + [j = y] a
@@ -682,13 +701,13 @@ __global__ void __launch_bounds__(LT) k_log_probs_grad_rows(LogProbGradArgs g, i
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const int j = first + u * (THREADS * V);
-        if (j <= g.numOut - V) v[u] = load_pack<T, V>(x + j);
+        if (j <= g.numOut - V) v[u] = load_pack<T, V>(x + j, g.nt);
         else {
 #pragma unroll
             for (int k = 0; k < V; ++k) v[u].v[k] = j < g.numOut - k ? x[j + k] : (T)0.f;
         }
         if (g.add) {
-            if (j <= g.numOut - V) t[u] = load_pack<T, V>(out + j);
+            if (j <= g.numOut - V) t[u] = load_pack<T, V>(out + j, g.nt);
             else {
 #pragma unroll
                 for (int k = 0; k < V; ++k) t[u].v[k] = j < g.numOut - k ? out[j + k] : (T)0.f;
@@ -708,7 +727,7 @@ __global__ void __launch_bounds__(LT) k_log_probs_grad_rows(LogProbGradArgs g, i
             if (g.add) y += (float)t[u].v[k];
             d.v[k] = (T)y;
         }
-        if (j <= g.numOut - V) store_pack<T, V>(out + j, d);
+        if (j <= g.numOut - V) store_pack<T, V>(out + j, d, g.nt);
         else {
 #pragma unroll
             for (int k = 0; k < V; ++k)
@@ -736,8 +755,8 @@ __global__ void __launch_bounds__(LT) k_log_probs_grad_cols(LogProbGradArgs g, i
         const T* from = x + (size_t)j * g.classStride;
         const T* prev = out + (size_t)j * g.targetClassStride;
         if (whole) {
-            v[u] = load_pack<T, P>(from);
-            if (g.add) t[u] = load_pack<T, P>(prev);
+            v[u] = load_pack<T, P>(from, g.nt);
+            if (g.add) t[u] = load_pack<T, P>(prev, g.nt);
         } else {
 #pragma unroll
             for (int k = 0; k < P; ++k) {
@@ -761,7 +780,7 @@ __global__ void __launch_bounds__(LT) k_log_probs_grad_cols(LogProbGradArgs g, i
             if (g.add) y += (float)t[u].v[k];
             d.v[k] = (T)y;
         }
-        if (whole) store_pack<T, P>(to, d);
+        if (whole) store_pack<T, P>(to, d, g.nt);
         else {
 #pragma unroll
             for (int k = 0; k < P; ++k)
@@ -822,9 +841,14 @@ Plan plan_log_probs(int type, int kinds, int numCases, int numOut, int numTop) {
     } else {
         p.P = numTop ? 4 : V;
         if (numCases < p.P) p.P = 1;
-        while (p.logG < 3 && (p.P << p.logG) < numCases) ++p.logG;
+        // A small matrix: every case in one part, if a workgroup of R classes by 1 ... 16 can hold it.  (Its lines are then read in short
+        // pieces, which the L2 makes up for; joining costs a launch.)
+        const bool small = (size_t)numCases * numOut * elem_size(type) <= (4u << 20) && numOut <= LT * 16;
+        for (p.U = small ? 1 : 16; small && LT * p.U < numOut; p.U *= 4) {}
+        while (p.logG < 3 && (p.P << p.logG) < numCases && (!small || (LT >> (p.logG + 1)) * p.U >= numOut)) ++p.logG;
         const int R = LT >> p.logG, tiles = ceil_div(numCases, p.P << p.logG);
-        for (p.U = 16; p.U > 1 && (numOut <= R * (p.U / 4) || (size_t)tiles * ceil_div(numOut, R * p.U) < 2 * (size_t)cus); p.U /= 4) {}
+        if (!small)
+            for (; p.U > 1 && (numOut <= R * (p.U / 4) || (size_t)tiles * ceil_div(numOut, R * p.U) < 2 * (size_t)cus); p.U /= 4) {}
         p.parts.span = R * p.U;
         p.parts.parts = ceil_div(numOut, p.parts.span);
         p.blocks = (size_t)tiles * p.parts.parts;
@@ -872,8 +896,8 @@ void launch_grad(const LogProbGradArgs& g, bool rows, hipStream_t s) {
             if (g.numOut <= 64 * V) hipLaunchKernelGGL((k_log_probs_grad_rows<T, 64, 1, ENT>), grid, block, 0, s, g, 1);
             else hipLaunchKernelGGL((k_log_probs_grad_rows<T, 64, 4, ENT>), grid, block, 0, s, g, 1);
         } else {
-            const int parts = ceil_div(g.numOut, LT * V * 4);
-            hipLaunchKernelGGL((k_log_probs_grad_rows<T, LT, 4, ENT>), dim3((unsigned)((size_t)g.numCases * parts)), block, 0, s, g, parts);
+            const int parts = ceil_div(g.numOut, LT * V * 2);
+            hipLaunchKernelGGL((k_log_probs_grad_rows<T, LT, 2, ENT>), dim3((unsigned)((size_t)g.numCases * parts)), block, 0, s, g, parts);
         }
         return;
     }
@@ -923,7 +947,7 @@ int mc_log_probs(const void* logits, int type, long long classStride, long long 
     p.parts.stats = static_cast<Part*>(workspace);
     p.parts.keys = reinterpret_cast<unsigned long long*>(p.parts.stats + (p.bytes ? (size_t)numCases * p.parts.parts : 0));
     const LogProbArgs a{logits, (size_t)classStride, (size_t)caseStride, labels, labelType, numCases, numOut, labelLogProbs, entropy, maxAndLogSum,
-                        topClasses, topLogProbs, numTop};
+                        topClasses, topLogProbs, numTop, streams((size_t)numCases * numOut * elem_size(type))};
     with_type(type, [&](auto t) {
         typedef decltype(t) T;
         if (numTop) launch_log_probs<T, true, true>(p, a, S(s));
@@ -959,7 +983,8 @@ int mc_log_probs_grad(const void* logits, int type, long long classStride, long 
     MC_REQUIRE(scaleEntropy == 0.f || entropy, "mc_log_probs_grad: the entropy's gradient needs the entropy");
     MC_REQUIRE(stream_on_current_device(s), "mc_log_probs_grad: the stream belongs to another device than the current one");
     const LogProbGradArgs a{logits, (size_t)classStride, (size_t)caseStride, labels, labelType, numCases, numOut, maxAndLogSum, entropy, gradLabel,
-                            gradEntropy, gradLogZ, scaleLabel, scaleEntropy, scaleLogZ, target, (size_t)targetClassStride, (size_t)targetCaseStride, add};
+                            gradEntropy, gradLogZ, scaleLabel, scaleEntropy, scaleLogZ, target, (size_t)targetClassStride, (size_t)targetCaseStride, add,
+                            streams((size_t)numCases * numOut * elem_size(type) * 2)};
     with_type(type, [&](auto t) {
         typedef decltype(t) T;
         if (scaleEntropy != 0.f) launch_grad<T, true>(a, kinds & targetKinds & BY_CASE, S(s));

@@ -5,6 +5,11 @@
 
 namespace mc {
 
+// A pointer that was itself loaded from memory, as one to global memory (the compiler would use flat accesses, which wait for the
+// scalar loads beside them).
+template <class T>
+using GlobalPtr = __attribute__((address_space(1))) T*;
+
 inline int elem_size(int type) { return type == MC_F32 ? 4 : 2; }
 inline bool float_type(int type) { return type == MC_F32 || type == MC_F16 || type == MC_BF16; }
 
@@ -12,8 +17,6 @@ inline bool float_type(int type) { return type == MC_F32 || type == MC_F16 || ty
 template <class T, int V>
 struct __attribute__((packed, aligned(sizeof(T)))) Pack { T v[V]; };
 
-// Streaming accesses: data that is read or written once and is larger than the caches.  (On 512 MiB: reads 6.9 TB/s against 6.3 with
-// ordinary loads, copies 6.2 against 5.8.)
 template <int BYTES, int ALIGN>
 struct Raw;   // BYTES bytes as a register vector, at any address that is a multiple of ALIGN (2 or 4)
 template <> struct Raw<16, 4> { typedef unsigned type __attribute__((ext_vector_type(4), aligned(4))); };
@@ -24,21 +27,82 @@ template <> struct Raw<4, 4> { typedef unsigned type; };
 template <> struct Raw<4, 2> { typedef unsigned type __attribute__((aligned(2))); };
 template <> struct Raw<2, 2> { typedef unsigned short type; };
 
+// Streaming accesses (nt) keep data that is read or written once, and is larger than the caches, from displacing the rest and themselves:
+// on 512 MiB reads reach 6.9 TB/s against 6.3 with ordinary loads, copies 6.2 against 5.8.  Data that fits the 256 MiB last-level cache
+// is better left to it: what the kernel before wrote is still there, and so is what the kernel after will read.
+inline bool streams(size_t bytes) { return bytes > ((size_t)192 << 20); }
+
 template <class T, int V>
-__device__ __forceinline__ Pack<T, V> load_pack(const T* p) {
+__device__ __forceinline__ Pack<T, V> load_pack(const T* p, bool nt) {
     typedef typename Raw<sizeof(T) * V, sizeof(T)>::type R;
-    const R r = __builtin_nontemporal_load(reinterpret_cast<const R*>(p));
+    const GlobalPtr<const R> q = (GlobalPtr<const R>)p;
+    const R r = nt ? __builtin_nontemporal_load(q) : *q;
     Pack<T, V> v;
     __builtin_memcpy(&v, &r, sizeof(v));
     return v;
 }
 template <class T, int V>
-__device__ __forceinline__ void store_pack(T* p, const Pack<T, V>& v) {
+__device__ __forceinline__ void store_pack(T* p, const Pack<T, V>& v, bool nt) {
     typedef typename Raw<sizeof(T) * V, sizeof(T)>::type R;
     R r;
     __builtin_memcpy(&r, &v, sizeof(v));
-    __builtin_nontemporal_store(r, reinterpret_cast<R*>(p));
+    if (nt) __builtin_nontemporal_store(r, (GlobalPtr<R>)p);
+    else *(GlobalPtr<R>)p = r;
 }
+
+// Elements stay in the registers that they were loaded into and are converted where they are used.  A Pass holds the constants that
+// takes, anew for each pass over them and hidden from the compiler, which would hold the converted values from one pass to the next
+// otherwise: twice the registers for 16-bit types.
+struct Pass {
+    unsigned high = 0xffff0000u, by = 16;
+    __device__ __forceinline__ Pass() { asm volatile("" : "+s"(high), "+s"(by)); }
+};
+// N elements of type T
+template <class T, int N>
+struct Words {
+    static constexpr int COUNT = N * sizeof(T) < 4 ? 1 : N * sizeof(T) / 4;
+    unsigned w[COUNT];
+    template <bool NT>
+    __device__ __forceinline__ void load(const T* p) {
+        typedef typename Raw<N * sizeof(T), sizeof(T)>::type R;
+        const GlobalPtr<const R> q = (GlobalPtr<const R>)p;
+        const R r = NT ? __builtin_nontemporal_load(q) : *q;
+        w[0] = 0;
+        __builtin_memcpy(w, &r, N * sizeof(T));
+    }
+    __device__ __forceinline__ void fill() {   // -inf
+        const unsigned inf = sizeof(T) == 4 ? 0xff800000u : __is_same(T, _Float16) ? 0xfc00fc00u : 0xff80ff80u;
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) w[i] = inf;
+    }
+    __device__ __forceinline__ void fill_first(int n) {   // -inf in the first n of them
+        const unsigned inf = sizeof(T) == 4 ? 0xff800000u : __is_same(T, _Float16) ? 0xfc00fc00u : 0xff80ff80u;
+        constexpr int PER = sizeof(T) == 4 ? 1 : 2;
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) {
+            if (PER == 2 && n == 2 * i + 1) w[i] = (w[i] & 0xffff0000u) | (inf & 0xffffu);
+            if (n >= PER * (i + 1)) w[i] = inf;
+        }
+    }
+    __device__ __forceinline__ void set(int k, T v) {
+        unsigned short h = 0;
+        if (sizeof(T) == 4) {
+            __builtin_memcpy(&w[k], &v, sizeof(T));
+            return;
+        }
+        __builtin_memcpy(&h, &v, 2);
+        w[k / 2] = k % 2 ? (w[k / 2] & 0xffffu) | (unsigned)h << 16 : (w[k / 2] & 0xffff0000u) | h;
+    }
+    __device__ __forceinline__ float at(int k, Pass p) const {
+        if (sizeof(T) == 4) return __uint_as_float(w[k]);
+        const unsigned u = w[k / 2];
+        if (__is_same(T, __bf16)) return __uint_as_float(k % 2 ? u & p.high : u << p.by);
+        const unsigned short h = (unsigned short)(k % 2 ? u >> p.by : u);
+        _Float16 v;
+        __builtin_memcpy(&v, &h, 2);
+        return (float)v;
+    }
+};
 
 // Calls f with a value of the element type that `type` names; false if it names none.
 template <class F>
