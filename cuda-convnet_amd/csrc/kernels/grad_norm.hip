@@ -26,6 +26,33 @@ __device__ __forceinline__ double block_sum(double v, double* sh) {
     return r;
 }
 
+// The squares of a pack.  Those of 16-bit numbers are exact in float32, and a tree of 8 of them is off by at most 3 half steps there: one
+// conversion to double for the pack, where the double pipe would take longer than the loads (2^28 bf16: 114 us in double throughout).
+// bf16 has float32's range, though: where the sum is infinite or might have lost bits below, doubles form it.
+template <class T, int V>
+__device__ __forceinline__ double pack_square(const Words<T, V>& x, Pass pass) {
+    if constexpr (sizeof(T) == 2) {
+        float p[V / 2];
+#pragma unroll
+        for (int k = 0; k < V / 2; ++k) {
+            const float a = x.at(2 * k, pass), b = x.at(2 * k + 1, pass);
+            p[k] = fmaf(b, b, a * a);
+        }
+#pragma unroll
+        for (int n = V / 4; n > 0; n /= 2)
+#pragma unroll
+            for (int k = 0; k < n; ++k) p[k] += p[k + n];
+        if (!__is_same(T, __bf16) || (p[0] > 0x1p-80f && p[0] < INFINITY)) return (double)p[0];
+    }
+    double s = 0.0;
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        const double d = (double)x.at(k, pass);
+        s += d * d;
+    }
+    return s;
+}
+
 // The packs of a span, U loads in flight a thread: past the end the last pack is loaded again and not counted.
 template <class T, bool NT>
 __device__ __forceinline__ double span_square(const T* g, unsigned n) {
@@ -39,12 +66,7 @@ __device__ __forceinline__ double span_square(const T* g, unsigned n) {
         const Pass pass;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            double s = 0.0;
-#pragma unroll
-            for (int k = 0; k < V; ++k) {
-                const double d = (double)x[u].at(k, pass);
-                s += d * d;
-            }
+            const double s = pack_square(x[u], pass);
             acc += at + u * GT < packs ? s : 0.0;
             asm volatile("" : "+v"(acc));   // one pack's doubles in registers at a time
         }
@@ -92,23 +114,35 @@ __global__ void __launch_bounds__(GT) k_grad_factor(const double* __restrict__ p
     }
 }
 
-// One pack of 4 elements a thread: a workgroup takes a quarter of a span.  (Streams of small tiles in the order of memory copy faster than
-// workgroups that walk through stretches of their own: 256 Mi elements bf16 -> float32 in 238 us against 281.)
+// kClipPacks packs of 4 elements a thread: a workgroup takes a part of a span.  (Streams of small tiles in the order of memory copy faster
+// than workgroups that walk through stretches of their own.)
+#ifndef CLIP_U
+#define CLIP_U 2
+#endif
+constexpr int kClipPacks = CLIP_U, kClipTile = GT * 4 * kClipPacks;
 template <class T, class O>
 __device__ __forceinline__ void tile_scale(const T* g, O* out, unsigned at, unsigned n, float f, bool nt) {
-    if (at + 4 <= n) {
-        const Pack<T, 4> x = load_pack<T, 4>(g + at, nt);
-        Pack<O, 4> y;
+    at += threadIdx.x * 4;
+    Pack<T, 4> x[kClipPacks];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) y.v[k] = f == 0.f ? (O)0.f : (O)((float)x.v[k] * f);
-        store_pack<O, 4>(out + at, y, nt);
-    } else
-        for (; at < n; ++at) {
-            const float x = (float)load_pack<T, 1>(g + at, false).v[0];
-            Pack<O, 1> y;
-            y.v[0] = f == 0.f ? (O)0.f : (O)(x * f);
-            store_pack<O, 1>(out + at, y, false);
-        }
+    for (int u = 0; u < kClipPacks; ++u)
+        if (at + u * GT * 4 + 4 <= n) x[u] = load_pack<T, 4>(g + at + u * GT * 4, nt);
+#pragma unroll
+    for (int u = 0; u < kClipPacks; ++u) {
+        unsigned j = at + u * GT * 4;
+        if (j + 4 <= n) {
+            Pack<O, 4> y;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) y.v[k] = f == 0.f ? (O)0.f : (O)((float)x[u].v[k] * f);
+            store_pack<O, 4>(out + j, y, nt);
+        } else
+            for (; j < n; ++j) {
+                const float v = (float)load_pack<T, 1>(g + j, false).v[0];
+                Pack<O, 1> y;
+                y.v[0] = f == 0.f ? (O)0.f : (O)(v * f);
+                store_pack<O, 1>(out + j, y, false);
+            }
+    }
 }
 template <class T>
 __device__ __forceinline__ void tile_clip(const mcGradSpan& sp, unsigned at, float f, bool nt) {
@@ -120,8 +154,8 @@ __device__ __forceinline__ void tile_clip(const mcGradSpan& sp, unsigned at, flo
 
 // Factor 0 writes zeros and not products: the gradients hold what made the norm infinite.
 __global__ void __launch_bounds__(GT) k_clip_grads(const mcGradSpan* __restrict__ spans, const float* __restrict__ normAndFactor, bool nt) {
-    const mcGradSpan sp = spans[blockIdx.x / (kSpan / (GT * 4))];
-    const unsigned at = (blockIdx.x % (kSpan / (GT * 4)) * GT + threadIdx.x) * 4;
+    const mcGradSpan sp = spans[blockIdx.x / (kSpan / kClipTile)];
+    const unsigned at = blockIdx.x % (kSpan / kClipTile) * kClipTile;
     if (at >= sp.count || !sp.out) return;
     const float f = normAndFactor[1] == 0.f ? 0.f : normAndFactor[1] * sp.scale;
     if (sp.out == sp.grad && f == 1.f) return;
@@ -137,43 +171,61 @@ __device__ __forceinline__ void step(float& w, float& i, float g, float f, float
     w += i;
 }
 // A workgroup takes a span, with up to 12 loads in flight a thread.
-__global__ void __launch_bounds__(GT) k_weights_update_clipped(float* w, float* inc, const float* __restrict__ grad, const mcUpdateSpan* __restrict__ spans,
+#ifndef UPD_U
+#define UPD_U 4
+#endif
+#ifndef UPD_P
+#define UPD_P 0
+#endif
+__global__ void __launch_bounds__(GT) k_weights_update_clipped(float* w, float* inc, const float* __restrict__ grad, const mcUpdateSpan* __restrict__ spans, int numSpans,
                                                                const float* __restrict__ normAndFactor, bool nt) {
-    const mcUpdateSpan sp = spans[blockIdx.x];
+    mcUpdateSpan next = spans[blockIdx.x];
     const float f = normAndFactor[1];
     if (f == 0.f) return;   // the norm is not finite: the step is dropped
+    for (int b = blockIdx.x; b < numSpans; b += gridDim.x) {
+    const mcUpdateSpan sp = next;
+    if (UPD_P) next = spans[min(b + (int)gridDim.x, numSpans - 1)];
     float *W = w + sp.start, *I = inc + sp.start;
     const float* G = grad + sp.start;
-    constexpr int U = 4;
-    unsigned v = 0;
-    for (; v + GT * 4 * U <= sp.count; v += GT * 4 * U) {
-        Pack<float, 4> ww[U], ii[U], gg[U];
+    constexpr int U = UPD_U;
+    const unsigned packs = sp.count / 4;
+    for (unsigned at = threadIdx.x; at - threadIdx.x < packs; at += GT * U) {
+        Words<float, 4> ww[U], ii[U], gg[U];
+        if (nt) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const unsigned at = v + (u * GT + threadIdx.x) * 4;
-            ww[u] = load_pack<float, 4>(W + at, nt);
-            ii[u] = load_pack<float, 4>(I + at, nt);
-            gg[u] = load_pack<float, 4>(G + at, nt);
+            for (int u = 0; u < U; ++u) {
+                const unsigned j = min(at + u * GT, packs - 1) * 4;
+                ww[u].load<true>(W + j);
+                ii[u].load<true>(I + j);
+                gg[u].load<true>(G + j);
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const unsigned j = min(at + u * GT, packs - 1) * 4;
+                ww[u].load<false>(W + j);
+                ii[u].load<false>(I + j);
+                gg[u].load<false>(G + j);
+            }
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const unsigned at = v + (u * GT + threadIdx.x) * 4;
+            Pack<float, 4> nw, ni;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) step(ww[u].v[k], ii[u].v[k], gg[u].v[k], f, sp.mom, sp.wceps);
-            store_pack<float, 4>(I + at, ii[u], nt);
-            store_pack<float, 4>(W + at, ww[u], nt);
+            for (int k = 0; k < 4; ++k) {
+                nw.v[k] = __uint_as_float(ww[u].w[k]);
+                ni.v[k] = __uint_as_float(ii[u].w[k]);
+                step(nw.v[k], ni.v[k], __uint_as_float(gg[u].w[k]), f, sp.mom, sp.wceps);
+            }
+            if (at + u * GT < packs) {
+                store_pack<float, 4>(I + (at + u * GT) * 4, ni, nt);
+                store_pack<float, 4>(W + (at + u * GT) * 4, nw, nt);
+            }
         }
     }
-    const unsigned end = sp.count / 4 * 4;
-    for (v += threadIdx.x * 4; v < end; v += GT * 4) {
-        Pack<float, 4> ww = load_pack<float, 4>(W + v, nt), ii = load_pack<float, 4>(I + v, nt);
-        const Pack<float, 4> gg = load_pack<float, 4>(G + v, nt);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) step(ww.v[k], ii.v[k], gg.v[k], f, sp.mom, sp.wceps);
-        store_pack<float, 4>(I + v, ii, nt);
-        store_pack<float, 4>(W + v, ww, nt);
+    const unsigned rest = packs * 4 + threadIdx.x;
+    if (rest < sp.count) step(W[rest], I[rest], G[rest], f, sp.mom, sp.wceps);
     }
-    if (end + threadIdx.x < sp.count) step(W[end + threadIdx.x], I[end + threadIdx.x], G[end + threadIdx.x], f, sp.mom, sp.wceps);
 }
 
 int partials_for(int numSpans) { return std::max(1, std::min(numSpans, kMaxPartials)); }
@@ -272,7 +324,7 @@ int mc_clip_grads(const mcGradSpan* spansDevice, int numSpans, const float* norm
     MC_REQUIRE(stream_on_current_device(s), "mc_clip_grads: the stream belongs to another device than the current one");
     if (numSpans == 0) return MC_OK;
     MC_REQUIRE(numSpans <= 0x1fffffff, "mc_clip_grads: too many spans");
-    hipLaunchKernelGGL(k_clip_grads, dim3(numSpans * (kSpan / (GT * 4))), dim3(GT), 0, S(s), spansDevice, normAndFactor, spans_stream(numSpans));
+    hipLaunchKernelGGL(k_clip_grads, dim3(numSpans * (kSpan / kClipTile)), dim3(GT), 0, S(s), spansDevice, normAndFactor, spans_stream(numSpans));
     return launch_status("mc_clip_grads");
 }
 
@@ -282,7 +334,7 @@ int mc_weights_update_spans_clipped(float* weights, float* inc, const float* gra
     MC_REQUIRE(aligned16(weights) && aligned16(inc) && aligned16(grad), "mc_weights_update_spans_clipped: arenas must be 16-byte aligned");
     MC_REQUIRE(stream_on_current_device(s), "mc_weights_update_spans_clipped: the stream belongs to another device than the current one");
     if (numSpans <= 0) return MC_OK;
-    hipLaunchKernelGGL(k_weights_update_clipped, dim3(numSpans), dim3(GT), 0, S(s), weights, inc, grad, spansDevice, normAndFactor,
+    hipLaunchKernelGGL(k_weights_update_clipped, dim3(UPD_P ? std::min(numSpans, UPD_P) : numSpans), dim3(GT), 0, S(s), weights, inc, grad, spansDevice, numSpans, normAndFactor,
                        spans_stream(numSpans));
     return launch_status("mc_weights_update_spans_clipped");
 }

@@ -446,6 +446,14 @@ __global__ void __launch_bounds__(LT) k_log_probs_cols(LogProbArgs a, Parts p, i
         for (int u = 0; u < U; ++u)
             if (lo + u * R + r >= hi) v[u].fill();
     }
+    // what the case's own thread will write: its way to memory (the label, then its logit) is begun now
+    const int mine = min((int)threadIdx.x, cases - 1), myCase = min((tile * G + mine / P) * P, a.numCases - P) + mine % P;
+    int label = -1;
+    float labelLogit = 0.f;
+    if (p.parts == 1 && a.labelLogProbs && (int)threadIdx.x < cases) {
+        label = label_of(a.labels, a.labelType, myCase, a.numOut);
+        if (label >= 0) labelLogit = (float)static_cast<const T*>(a.logits)[(size_t)label * a.classStride + (size_t)myCase * a.caseStride];
+    }
     float pm[TOP ? WINDOWS : 1][P], m[P], s[P], w[P];
     const Pass first;
 #pragma unroll
@@ -498,14 +506,12 @@ __global__ void __launch_bounds__(LT) k_log_probs_cols(LogProbArgs a, Parts p, i
     }
     __syncthreads();
     if ((int)threadIdx.x < cases) {
-        const int cc = threadIdx.x, n = min((tile * G + cc / P) * P, a.numCases - P) + cc % P;
+        const int cc = threadIdx.x, n = myCase;
         float M = fmaxf(fmaxf(shM[0][cc], shM[1][cc]), fmaxf(shM[2][cc], shM[3][cc]));
         float S = shS[0][cc] + shS[1][cc] + shS[2][cc] + shS[3][cc], Wt = shW[0][cc] + shW[1][cc] + shW[2][cc] + shW[3][cc];
         take_back(M, S, Wt);
         if (p.parts == 1) {
             const CaseStats c = case_stats(M, S);
-            const int label = a.labelLogProbs ? label_of(a.labels, a.labelType, n, a.numOut) : -1;
-            const float labelLogit = label >= 0 ? (float)static_cast<const T*>(a.logits)[(size_t)label * a.classStride + (size_t)n * a.caseStride] : 0.f;
             write_case(a, n, c, S, Wt, label, labelLogit);
             if (TOP) {
                 shS[0][cc] = c.logSum;   // (these two are read by their own thread only until the next barrier)
@@ -525,8 +531,8 @@ __global__ void __launch_bounds__(LT) k_log_probs_cols(LogProbArgs a, Parts p, i
             q[i] = owner < cases && at < stretches ? shSeg[owner * (stretches + 1) + at] : -INFINITY;
         }
         const unsigned long long mask = (lanes == 64 ? ~0ull : (1ull << lanes) - 1) << (lane - lane % lanes);
-        const int mine = min(owner, cases - 1);
-        const float most = fmaxf(fmaxf(shM[0][mine], shM[1][mine]), fmaxf(shM[2][mine], shM[3][mine]));
+        const int own = min(owner, cases - 1);
+        const float most = fmaxf(fmaxf(shM[0][own], shM[1][own]), fmaxf(shM[2][own], shM[3][own]));
         const float tau = hi - lo <= kFewClasses / 2 ? -INFINITY : top_threshold(q, a.numTop, most, mask);
         if (owner < cases && sub == 0) shTau[owner] = tau;
     }
@@ -579,19 +585,36 @@ __global__ void __launch_bounds__(LT) k_log_probs_join(LogProbArgs a, Parts p) {
     const size_t row = (size_t)blockIdx.x * GROUPS + group;
     if (row >= (size_t)a.numCases) return;
     const int n = (int)row;
-    const int label = a.labelLogProbs ? label_of(a.labels, a.labelType, n, a.numOut) : -1;
+    // All that is read is under way before anything is waited for: statistics, label (and then its logit), the parts' best keys, and as many
+    // of all keys as the threads hold at EARLY each.
+    constexpr int EARLY = 6;
     const Part* stats = p.stats + row * p.parts;
+    const unsigned long long* keys = p.keys + row * p.parts * a.numTop;
+    const int total = p.parts * a.numTop;
+    Part part = {-INFINITY, 0.f, 0.f, 0.f};
+    if (tid < p.parts) part = stats[tid];
+    int label = -1;
+    if (a.labelLogProbs) label = label_of(a.labels, a.labelType, n, a.numOut);
+    unsigned long long early[EARLY];
+#pragma unroll
+    for (int i = 0; i < EARLY; ++i) early[i] = tid + i * THREADS < total ? keys[tid + i * THREADS] : 0;
+    const bool thresholds = p.parts > a.numTop && total > kFewClasses;
+    constexpr int Q = 8;
+    unsigned long long head[Q];
+    const int heads = min(p.parts, 64 * Q);   // (beyond: the first ones' threshold holds too)
+#pragma unroll
+    for (int i = 0; i < Q; ++i) head[i] = thresholds && (int)(threadIdx.x & 63) + 64 * i < heads ? keys[(size_t)((threadIdx.x & 63) + 64 * i) * a.numTop] : 0;
     const float labelLogit = label >= 0 ? (float)static_cast<const T*>(a.logits)[(size_t)label * a.classStride + row * a.caseStride] : 0.f;
     if (tid == 0) shCount[group] = 0;
-    float m = -INFINITY;
-    for (int i = tid; i < p.parts; i += THREADS) m = fmaxf(m, stats[i].m);
+    float m = part.m;
+    for (int i = tid + THREADS; i < p.parts; i += THREADS) m = fmaxf(m, stats[i].m);
     m = G::max(m, shRed[group]);
     float s = 0.f, w = 0.f;
     for (int i = tid; i < p.parts; i += THREADS) {
-        const Part q = stats[i];
-        const float d = q.m == m ? 0.f : (q.m - m) * kLog2e, f = __builtin_amdgcn_exp2f(d);
-        s += q.s * f;
-        w += fmaf(fmaxf(d, -200.f), q.s, q.w) * f;
+        if (i != tid) part = stats[i];
+        const float d = part.m == m ? 0.f : (part.m - m) * kLog2e, f = __builtin_amdgcn_exp2f(d);
+        s += part.s * f;
+        w += fmaf(fmaxf(d, -200.f), part.s, part.w) * f;
     }
     G::sum2(s, w, shRed[group] + G::WAVES);
     const CaseStats c = case_stats(m, s);
@@ -599,29 +622,23 @@ __global__ void __launch_bounds__(LT) k_log_probs_join(LogProbArgs a, Parts p) {
     if (!a.numTop) return;
 
     // candidates: keys that reach a value that numTop parts' best keys reach
-    const unsigned long long* keys = p.keys + row * p.parts * a.numTop;
     float threshold = -INFINITY;
-    if (p.parts > a.numTop && p.parts * a.numTop > kFewClasses) {
-        constexpr int Q = 8;
+    if (thresholds) {
         float q[Q];
-        const int parts = min(p.parts, 64 * Q);   // (beyond: the first ones' threshold holds too)
 #pragma unroll
-        for (int i = 0; i < Q; ++i) {
-            const int at = (threadIdx.x & 63) + 64 * i;
-            const unsigned long long key = at < parts ? keys[(size_t)at * a.numTop] : 0;
-            q[i] = key ? key_logit(key) : -INFINITY;
-        }
+        for (int i = 0; i < Q; ++i) q[i] = head[i] ? key_logit(head[i]) : -INFINITY;
         threshold = top_threshold(q, a.numTop, m, ~0ull);
     }
-    const int total = p.parts * a.numTop;
-    G::sync();
-    for (int i = tid; i < total; i += THREADS) {
-        const unsigned long long key = keys[i];
+    const auto take = [&](unsigned long long key) {
         if (key && key_logit(key) >= threshold) {
             const int to = atomicAdd(&shCount[group], 1);
             if (to < CAND) shCand[group][to] = key;
         }
-    }
+    };
+    G::sync();
+#pragma unroll
+    for (int i = 0; i < EARLY; ++i) take(early[i]);
+    for (int i = tid + EARLY * THREADS; i < total; i += THREADS) take(keys[i]);
     G::sync();
     const int count = shCount[group];
     if (count <= CAND) {
@@ -687,52 +704,55 @@ __device__ __forceinline__ float grad_of(float x, const CaseGrad& c) {
     return ENT ? p * fmaf(-c.h, fmaxf(lp, -200.f) + c.H, c.A) : p * c.A;
 }
 
-template <class T, int THREADS, int U, bool ENT>
+// The gradient of a pack (and, with add, of what the target holds), element by element.  y: the label's place in the pack, if it is in it.
+template <bool ENT, class T, int N>
+__device__ __forceinline__ Pack<T, N> grad_pack(const Words<T, N>& v, const Words<T, N>& t, bool add, const CaseGrad& c, int y, Pass pass) {
+    Pack<T, N> d;
+    const bool here = (unsigned)y < (unsigned)N;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        float x = grad_of<ENT>(v.at(k, pass), c);
+        if (here && y == k) x += c.a;
+        if (add) x += t.at(k, pass);
+        d.v[k] = (T)x;
+    }
+    return d;
+}
+
+template <class T, int THREADS, int U, bool ENT, bool NT>
 __global__ void __launch_bounds__(LT) k_log_probs_grad_rows(LogProbGradArgs g, int parts) {
+    typedef Group<THREADS> G;
     constexpr int V = 16 / sizeof(T), GROUPS = LT / THREADS;
-    const size_t item = (size_t)blockIdx.x * GROUPS + threadIdx.x / THREADS;
-    const size_t row = item / parts;
-    if (row >= (size_t)g.numCases) return;
-    const int lo = (int)(item - row * parts) * (THREADS * U * V);
-    const T* x = static_cast<const T*>(g.logits) + row * g.caseStride;
-    T* out = static_cast<T*>(g.target) + row * g.targetCaseStride;
-    const int first = lo + (threadIdx.x & (THREADS - 1)) * V;
-    Pack<T, V> v[U], t[U];
+    const unsigned item = blockIdx.x * GROUPS + G::index(), row = item / (unsigned)parts;
+    if (row >= (unsigned)g.numCases) return;
+    const int lo = (int)(item - row * parts) * (THREADS * U * V), len = g.numOut - lo;
+    const T* x = static_cast<const T*>(g.logits) + row * g.caseStride + lo;
+    T* out = static_cast<T*>(g.target) + row * g.targetCaseStride + lo;
+    const int first = G::tid() * V, last = len - V;
+    const Pass pass;
+    if (last >= 0) {   // whole packs; those past the end read the last one and write nothing
+        Words<T, V> v[U], t[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const int j = first + u * (THREADS * V);
-        if (j <= g.numOut - V) v[u] = load_pack<T, V>(x + j, g.nt);
-        else {
-#pragma unroll
-            for (int k = 0; k < V; ++k) v[u].v[k] = j < g.numOut - k ? x[j + k] : (T)0.f;
-        }
+        for (int u = 0; u < U; ++u) v[u].template load<NT>(x + (unsigned)min(first + u * (THREADS * V), last));
         if (g.add) {
-            if (j <= g.numOut - V) t[u] = load_pack<T, V>(out + j, g.nt);
-            else {
 #pragma unroll
-                for (int k = 0; k < V; ++k) t[u].v[k] = j < g.numOut - k ? out[j + k] : (T)0.f;
-            }
+            for (int u = 0; u < U; ++u) t[u].template load<NT>(out + (unsigned)min(first + u * (THREADS * V), last));
+        }
+        const CaseGrad c = case_grad<ENT>(g, (int)row);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int j = first + u * (THREADS * V);
+            const Pack<T, V> d = grad_pack<ENT>(v[u], t[u], g.add, c, c.y - lo - j, pass);
+            if (j <= last) store_pack<T, V>(out + (unsigned)j, d, NT);
         }
     }
-    const CaseGrad c = case_grad<ENT>(g, (int)row);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const int j = first + u * (THREADS * V);
-        Pack<T, V> d;
-        const bool here = (unsigned)(c.y - j) < (unsigned)V;
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-            float y = grad_of<ENT>((float)v[u].v[k], c);
-            if (here && c.y == j + k) y += c.a;
-            if (g.add) y += (float)t[u].v[k];
-            d.v[k] = (T)y;
-        }
-        if (j <= g.numOut - V) store_pack<T, V>(out + j, d, g.nt);
-        else {
-#pragma unroll
-            for (int k = 0; k < V; ++k)
-                if (j < g.numOut - k) out[j + k] = d.v[k];
-        }
+    const int rest = len % V, at = len - rest + G::tid();   // the case's last classes, where they fill no pack
+    if (len <= THREADS * U * V && G::tid() < rest) {
+        const CaseGrad c = case_grad<ENT>(g, (int)row);
+        Words<T, 1> v, t;
+        v.template load<false>(x + at);
+        if (g.add) t.template load<false>(out + at);
+        store_pack<T, 1>(out + at, grad_pack<ENT>(v, t, g.add, c, c.y - lo - at, pass), false);
     }
 }
 
@@ -832,7 +852,7 @@ Plan plan_log_probs(int type, int kinds, int numCases, int numOut, int numTop) {
             p.blocks = ceil_div(numCases, LT / 64);
         } else {
             p.threads = LT;
-            for (p.U = 16; p.U > 1 && (size_t)numCases * ceil_div(numOut, LT * V * p.U) < 2 * (size_t)cus; p.U /= 4) {}
+            for (p.U = 16; p.U > 1 && (size_t)numCases * ceil_div(numOut, LT * V * p.U) < (p.U == 16 ? 4 : 1) * (size_t)cus; p.U /= 4) {}
             p.parts.parts = ceil_div(numOut, LT * V * p.U);
             p.parts.span = ceil_div(ceil_div(numOut, p.parts.parts), V) * V;
             p.parts.parts = ceil_div(numOut, p.parts.span);
@@ -886,27 +906,33 @@ void launch_log_probs(const Plan& p, const LogProbArgs& a, hipStream_t s) {
     else hipLaunchKernelGGL((k_log_probs_join<T, LT>), dim3(a.numCases), dim3(LT), 0, s, a, p.parts);
 }
 
+template <class T, bool ENT, bool NT>
+void launch_grad_rows(const LogProbGradArgs& g, hipStream_t s) {
+    constexpr int V = 16 / (int)sizeof(T), U = 4;
+    const dim3 block(LT);
+    if (g.numOut <= 64 * V * U) {
+        const dim3 grid(ceil_div(g.numCases, LT / 64));
+        if (g.numOut <= 64 * V) hipLaunchKernelGGL((k_log_probs_grad_rows<T, 64, 1, ENT, NT>), grid, block, 0, s, g, 1);
+        else hipLaunchKernelGGL((k_log_probs_grad_rows<T, 64, U, ENT, NT>), grid, block, 0, s, g, 1);
+    } else {
+        const int parts = ceil_div(g.numOut, LT * V * U);
+        hipLaunchKernelGGL((k_log_probs_grad_rows<T, LT, U, ENT, NT>), dim3((unsigned)((size_t)g.numCases * parts)), block, 0, s, g, parts);
+    }
+}
 template <class T, bool ENT>
 void launch_grad(const LogProbGradArgs& g, bool rows, hipStream_t s) {
     constexpr int V = 16 / (int)sizeof(T);
-    const dim3 block(LT);
     if (rows) {
-        if (g.numOut <= 64 * V * 4) {
-            const dim3 grid(ceil_div(g.numCases, LT / 64));
-            if (g.numOut <= 64 * V) hipLaunchKernelGGL((k_log_probs_grad_rows<T, 64, 1, ENT>), grid, block, 0, s, g, 1);
-            else hipLaunchKernelGGL((k_log_probs_grad_rows<T, 64, 4, ENT>), grid, block, 0, s, g, 1);
-        } else {
-            const int parts = ceil_div(g.numOut, LT * V * 2);
-            hipLaunchKernelGGL((k_log_probs_grad_rows<T, LT, 2, ENT>), dim3((unsigned)((size_t)g.numCases * parts)), block, 0, s, g, parts);
-        }
+        if (g.nt) launch_grad_rows<T, ENT, true>(g, s);
+        else launch_grad_rows<T, ENT, false>(g, s);
         return;
     }
     int logG = 0;
     const int P = g.numCases < V ? 1 : V;
     while (logG < 4 && (P << logG) < g.numCases) ++logG;
-    const unsigned blocks = (unsigned)((size_t)ceil_div(g.numCases, P << logG) * ceil_div(g.numOut, (LT >> logG) * 4));
-    if (P == 1) hipLaunchKernelGGL((k_log_probs_grad_cols<T, 1, 4, ENT>), dim3(blocks), block, 0, s, g, logG);
-    else hipLaunchKernelGGL((k_log_probs_grad_cols<T, V, 4, ENT>), dim3(blocks), block, 0, s, g, logG);
+    const dim3 block(LT), grid((unsigned)((size_t)ceil_div(g.numCases, P << logG) * ceil_div(g.numOut, (LT >> logG) * 4)));
+    if (P == 1) hipLaunchKernelGGL((k_log_probs_grad_cols<T, 1, 4, ENT>), grid, block, 0, s, g, logG);
+    else hipLaunchKernelGGL((k_log_probs_grad_cols<T, V, 4, ENT>), grid, block, 0, s, g, logG);
 }
 
 }  // namespace
