@@ -72,7 +72,7 @@ __device__ __forceinline__ double span_square(const T* g, unsigned n) {
         }
     }
     if (threadIdx.x < n - packs * V) {
-        const double d = (double)(float)load_pack<T, 1>(g + packs * V + threadIdx.x, NT).v[0];
+        const double d = (double)(float)load_pack<NT, T, 1>(g + packs * V + threadIdx.x).v[0];
         acc += d * d;
     }
     return acc;
@@ -116,17 +116,14 @@ __global__ void __launch_bounds__(GT) k_grad_factor(const double* __restrict__ p
 
 // kClipPacks packs of 4 elements a thread: a workgroup takes a part of a span.  (Streams of small tiles in the order of memory copy faster
 // than workgroups that walk through stretches of their own.)
-#ifndef CLIP_U
-#define CLIP_U 2
-#endif
-constexpr int kClipPacks = CLIP_U, kClipTile = GT * 4 * kClipPacks;
-template <class T, class O>
-__device__ __forceinline__ void tile_scale(const T* g, O* out, unsigned at, unsigned n, float f, bool nt) {
+constexpr int kClipPacks = 2, kClipTile = GT * 4 * kClipPacks;
+template <bool NT, class T, class O>
+__device__ __forceinline__ void tile_scale(const T* g, O* out, unsigned at, unsigned n, float f) {
     at += threadIdx.x * 4;
     Pack<T, 4> x[kClipPacks];
 #pragma unroll
     for (int u = 0; u < kClipPacks; ++u)
-        if (at + u * GT * 4 + 4 <= n) x[u] = load_pack<T, 4>(g + at + u * GT * 4, nt);
+        if (at + u * GT * 4 + 4 <= n) x[u] = load_pack<NT, T, 4>(g + at + u * GT * 4);
 #pragma unroll
     for (int u = 0; u < kClipPacks; ++u) {
         unsigned j = at + u * GT * 4;
@@ -134,34 +131,35 @@ __device__ __forceinline__ void tile_scale(const T* g, O* out, unsigned at, unsi
             Pack<O, 4> y;
 #pragma unroll
             for (int k = 0; k < 4; ++k) y.v[k] = f == 0.f ? (O)0.f : (O)((float)x[u].v[k] * f);
-            store_pack<O, 4>(out + j, y, nt);
+            store_pack<NT, O, 4>(out + j, y);
         } else
             for (; j < n; ++j) {
-                const float v = (float)load_pack<T, 1>(g + j, false).v[0];
+                const float v = (float)load_pack<false, T, 1>(g + j).v[0];
                 Pack<O, 1> y;
                 y.v[0] = f == 0.f ? (O)0.f : (O)(v * f);
-                store_pack<O, 1>(out + j, y, false);
+                store_pack<false, O, 1>(out + j, y);
             }
     }
 }
-template <class T>
-__device__ __forceinline__ void tile_clip(const mcGradSpan& sp, unsigned at, float f, bool nt) {
+template <bool NT, class T>
+__device__ __forceinline__ void tile_clip(const mcGradSpan& sp, unsigned at, float f) {
     const T* g = static_cast<const T*>(sp.grad);
-    if (sp.outType == MC_F32) tile_scale(g, static_cast<float*>(sp.out), at, sp.count, f, nt);
-    else if (sp.outType == MC_F16) tile_scale(g, static_cast<_Float16*>(sp.out), at, sp.count, f, nt);
-    else tile_scale(g, static_cast<__bf16*>(sp.out), at, sp.count, f, nt);
+    if (sp.outType == MC_F32) tile_scale<NT>(g, static_cast<float*>(sp.out), at, sp.count, f);
+    else if (sp.outType == MC_F16) tile_scale<NT>(g, static_cast<_Float16*>(sp.out), at, sp.count, f);
+    else tile_scale<NT>(g, static_cast<__bf16*>(sp.out), at, sp.count, f);
 }
 
 // Factor 0 writes zeros and not products: the gradients hold what made the norm infinite.
-__global__ void __launch_bounds__(GT) k_clip_grads(const mcGradSpan* __restrict__ spans, const float* __restrict__ normAndFactor, bool nt) {
+template <bool NT>
+__global__ void __launch_bounds__(GT) k_clip_grads(const mcGradSpan* __restrict__ spans, const float* __restrict__ normAndFactor) {
     const mcGradSpan sp = spans[blockIdx.x / (kSpan / kClipTile)];
     const unsigned at = blockIdx.x % (kSpan / kClipTile) * kClipTile;
     if (at >= sp.count || !sp.out) return;
     const float f = normAndFactor[1] == 0.f ? 0.f : normAndFactor[1] * sp.scale;
     if (sp.out == sp.grad && f == 1.f) return;
-    if (sp.gradType == MC_F32) tile_clip<float>(sp, at, f, nt);
-    else if (sp.gradType == MC_F16) tile_clip<_Float16>(sp, at, f, nt);
-    else tile_clip<__bf16>(sp, at, f, nt);
+    if (sp.gradType == MC_F32) tile_clip<NT, float>(sp, at, f);
+    else if (sp.gradType == MC_F16) tile_clip<NT, _Float16>(sp, at, f);
+    else tile_clip<NT, __bf16>(sp, at, f);
 }
 
 // inc = mom*inc + factor*grad; inc += wceps*W; W += inc, in the order (and, at factor 1, with the bits) of mc_weights_update_spans.
@@ -171,42 +169,24 @@ __device__ __forceinline__ void step(float& w, float& i, float g, float f, float
     w += i;
 }
 // A workgroup takes a span, with up to 12 loads in flight a thread.
-#ifndef UPD_U
-#define UPD_U 4
-#endif
-#ifndef UPD_P
-#define UPD_P 0
-#endif
-__global__ void __launch_bounds__(GT) k_weights_update_clipped(float* w, float* inc, const float* __restrict__ grad, const mcUpdateSpan* __restrict__ spans, int numSpans,
-                                                               const float* __restrict__ normAndFactor, bool nt) {
-    mcUpdateSpan next = spans[blockIdx.x];
+template <bool NT>
+__global__ void __launch_bounds__(GT) __attribute__((amdgpu_waves_per_eu(8)))
+k_weights_update_clipped(float* w, float* inc, const float* __restrict__ grad, const mcUpdateSpan* __restrict__ spans, const float* __restrict__ normAndFactor) {
+    const mcUpdateSpan sp = spans[blockIdx.x];
     const float f = normAndFactor[1];
     if (f == 0.f) return;   // the norm is not finite: the step is dropped
-    for (int b = blockIdx.x; b < numSpans; b += gridDim.x) {
-    const mcUpdateSpan sp = next;
-    if (UPD_P) next = spans[min(b + (int)gridDim.x, numSpans - 1)];
     float *W = w + sp.start, *I = inc + sp.start;
     const float* G = grad + sp.start;
-    constexpr int U = UPD_U;
+    constexpr int U = 4;
     const unsigned packs = sp.count / 4;
-    for (unsigned at = threadIdx.x; at - threadIdx.x < packs; at += GT * U) {
+    for (unsigned at = threadIdx.x; at - threadIdx.x < packs; at += GT * U) {   // past the end the last pack is loaded again, and not stored
         Words<float, 4> ww[U], ii[U], gg[U];
-        if (nt) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const unsigned j = min(at + u * GT, packs - 1) * 4;
-                ww[u].load<true>(W + j);
-                ii[u].load<true>(I + j);
-                gg[u].load<true>(G + j);
-            }
-        } else {
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const unsigned j = min(at + u * GT, packs - 1) * 4;
-                ww[u].load<false>(W + j);
-                ii[u].load<false>(I + j);
-                gg[u].load<false>(G + j);
-            }
+        for (int u = 0; u < U; ++u) {
+            const unsigned j = min(at + u * GT, packs - 1) * 4;
+            ww[u].load<NT>(W + j);
+            ii[u].load<NT>(I + j);
+            gg[u].load<NT>(G + j);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -218,14 +198,13 @@ __global__ void __launch_bounds__(GT) k_weights_update_clipped(float* w, float* 
                 step(nw.v[k], ni.v[k], __uint_as_float(gg[u].w[k]), f, sp.mom, sp.wceps);
             }
             if (at + u * GT < packs) {
-                store_pack<float, 4>(I + (at + u * GT) * 4, ni, nt);
-                store_pack<float, 4>(W + (at + u * GT) * 4, nw, nt);
+                store_pack<NT, float, 4>(I + (at + u * GT) * 4, ni);
+                store_pack<NT, float, 4>(W + (at + u * GT) * 4, nw);
             }
         }
     }
     const unsigned rest = packs * 4 + threadIdx.x;
     if (rest < sp.count) step(W[rest], I[rest], G[rest], f, sp.mom, sp.wceps);
-    }
 }
 
 int partials_for(int numSpans) { return std::max(1, std::min(numSpans, kMaxPartials)); }
@@ -298,8 +277,9 @@ int mc_grad_spans(const mcGradTensor* tensors, int numTensors, mcGradSpan* spans
     return MC_OK;
 }
 
-// Spans are nearly all of kSpan elements where there are so many that streaming pays.
-static bool spans_stream(int numSpans) { return streams((size_t)numSpans * kSpan * 2); }
+// Spans are nearly all of kSpan elements where there are so many that streaming pays, and what a step touches besides the gradients is
+// about as much again (norm and update after a pass that wrote the gradients: 2^24 elements 87 us without and 92 with nt, 2^25 187 and 173).
+static bool spans_stream(int numSpans) { return streams((size_t)numSpans * kSpan * 8); }
 
 size_t mc_grad_norm_workspace_bytes(int numSpans) { return (size_t)partials_for(numSpans) * sizeof(double); }
 
@@ -324,7 +304,9 @@ int mc_clip_grads(const mcGradSpan* spansDevice, int numSpans, const float* norm
     MC_REQUIRE(stream_on_current_device(s), "mc_clip_grads: the stream belongs to another device than the current one");
     if (numSpans == 0) return MC_OK;
     MC_REQUIRE(numSpans <= 0x1fffffff, "mc_clip_grads: too many spans");
-    hipLaunchKernelGGL(k_clip_grads, dim3(numSpans * (kSpan / kClipTile)), dim3(GT), 0, S(s), spansDevice, normAndFactor, spans_stream(numSpans));
+    const dim3 grid(numSpans * (kSpan / kClipTile)), block(GT);
+    if (spans_stream(numSpans)) hipLaunchKernelGGL(k_clip_grads<true>, grid, block, 0, S(s), spansDevice, normAndFactor);
+    else hipLaunchKernelGGL(k_clip_grads<false>, grid, block, 0, S(s), spansDevice, normAndFactor);
     return launch_status("mc_clip_grads");
 }
 
@@ -334,8 +316,8 @@ int mc_weights_update_spans_clipped(float* weights, float* inc, const float* gra
     MC_REQUIRE(aligned16(weights) && aligned16(inc) && aligned16(grad), "mc_weights_update_spans_clipped: arenas must be 16-byte aligned");
     MC_REQUIRE(stream_on_current_device(s), "mc_weights_update_spans_clipped: the stream belongs to another device than the current one");
     if (numSpans <= 0) return MC_OK;
-    hipLaunchKernelGGL(k_weights_update_clipped, dim3(UPD_P ? std::min(numSpans, UPD_P) : numSpans), dim3(GT), 0, S(s), weights, inc, grad, spansDevice, numSpans, normAndFactor,
-                       spans_stream(numSpans));
+    if (spans_stream(numSpans)) hipLaunchKernelGGL(k_weights_update_clipped<true>, dim3(numSpans), dim3(GT), 0, S(s), weights, inc, grad, spansDevice, normAndFactor);
+    else hipLaunchKernelGGL(k_weights_update_clipped<false>, dim3(numSpans), dim3(GT), 0, S(s), weights, inc, grad, spansDevice, normAndFactor);
     return launch_status("mc_weights_update_spans_clipped");
 }
 

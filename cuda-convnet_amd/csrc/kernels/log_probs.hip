@@ -4,6 +4,7 @@
 // and (m, s, w) of two sets of classes join into those of their union, so a case may be split over workgroups.
 #include <math.h>
 #include <algorithm>
+#include <type_traits>
 #include "mc_types.h"
 
 namespace mc {
@@ -23,7 +24,6 @@ struct LogProbArgs {
     int* topClasses;
     float* topLogProbs;
     int numTop;
-    bool nt;                      // the logits are read past the caches
 };
 
 // What a workgroup leaves of its classes of a case for the joining kernel; its best numTop keys follow in an array of their own.
@@ -288,7 +288,7 @@ __device__ __forceinline__ float shifted(const Words<T, N>& v, int k, Shift h, P
 // A workgroup (or wave) takes up to THREADS * U packs of 16 bytes of one case into registers in one burst of loads, and does all the
 // rest there: the largest logit, the sums against it, the candidates for the top.
 constexpr int kPacks = 128;
-template <class T, int THREADS, int U, bool ENT, bool TOP>
+template <class T, int THREADS, int U, bool ENT, bool TOP, bool NT>
 __global__ void __launch_bounds__(LT) __attribute__((amdgpu_waves_per_eu(4))) k_log_probs_rows(LogProbArgs a, Parts p) {
     typedef Group<THREADS> G;
     constexpr int V = 16 / sizeof(T), GROUPS = LT / THREADS;
@@ -315,13 +315,8 @@ __global__ void __launch_bounds__(LT) __attribute__((amdgpu_waves_per_eu(4))) k_
     const bool whole = THREADS == LT || a.numOut >= V;
     if (whole) {
         const T* from = x - back;
-        if (a.nt) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) v[u].template load<true>(from + (unsigned)(min(first + u * (THREADS * V), last) + back));
-        } else {
-#pragma unroll
-            for (int u = 0; u < U; ++u) v[u].template load<false>(from + (unsigned)(min(first + u * (THREADS * V), last) + back));
-        }
+        for (int u = 0; u < U; ++u) v[u].template load<NT>(from + (unsigned)(min(first + u * (THREADS * V), last) + back));
         if (len != THREADS * U * V) {
 #pragma unroll
             for (int u = 0; u < U; ++u) v[u].fill_first(first + u * (THREADS * V) - last);
@@ -418,7 +413,7 @@ __host__ __device__ constexpr int col_list_keys(int cases) { return cases * kCol
 constexpr size_t col_lds_bytes(int cases, int stretches) {
     return col_list_keys(cases) * sizeof(unsigned long long) + ((size_t)cases * (stretches + 1) + 2 * cases) * sizeof(float);
 }
-template <class T, int P, int U, bool ENT, bool TOP>
+template <class T, int P, int U, bool ENT, bool TOP, bool NT>
 __global__ void __launch_bounds__(LT) k_log_probs_cols(LogProbArgs a, Parts p, int logG) {
     constexpr int W = U >= 4 ? U / 4 : 1, WINDOWS = U / W;   // the top's maxima are kept for W classes at a time
     constexpr int Q = P == 1 ? 16 : WINDOWS * P;
@@ -434,13 +429,8 @@ __global__ void __launch_bounds__(LT) k_log_probs_cols(LogProbArgs a, Parts p, i
     const T* x = static_cast<const T*>(a.logits) + (size_t)n0 * (P == 1 ? a.caseStride : 1);
 
     Words<T, P> v[U];
-    if (a.nt) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) v[u].template load<true>(x + (size_t)min(lo + u * R + r, hi - 1) * a.classStride);
-    } else {
-#pragma unroll
-        for (int u = 0; u < U; ++u) v[u].template load<false>(x + (size_t)min(lo + u * R + r, hi - 1) * a.classStride);
-    }
+    for (int u = 0; u < U; ++u) v[u].template load<NT>(x + (size_t)min(lo + u * R + r, hi - 1) * a.classStride);
     if (hi - lo != U * R) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -677,7 +667,6 @@ struct LogProbGradArgs {
     void* target;
     size_t targetClassStride, targetCaseStride;
     int add;
-    bool nt;
 };
 
 // d_j = p_j (A - h (ln p_j + H)) + [j = y] a
@@ -743,7 +732,7 @@ __global__ void __launch_bounds__(LT) k_log_probs_grad_rows(LogProbGradArgs g, i
         for (int u = 0; u < U; ++u) {
             const int j = first + u * (THREADS * V);
             const Pack<T, V> d = grad_pack<ENT>(v[u], t[u], g.add, c, c.y - lo - j, pass);
-            if (j <= last) store_pack<T, V>(out + (unsigned)j, d, NT);
+            if (j <= last) store_pack<NT, T, V>(out + (unsigned)j, d);
         }
     }
     const int rest = len % V, at = len - rest + G::tid();   // the case's last classes, where they fill no pack
@@ -752,61 +741,51 @@ __global__ void __launch_bounds__(LT) k_log_probs_grad_rows(LogProbGradArgs g, i
         Words<T, 1> v, t;
         v.template load<false>(x + at);
         if (g.add) t.template load<false>(out + at);
-        store_pack<T, 1>(out + at, grad_pack<ENT>(v, t, g.add, c, c.y - lo - at, pass), false);
+        store_pack<false, T, 1>(out + at, grad_pack<ENT>(v, t, g.add, c, c.y - lo - at, pass));
     }
 }
 
-template <class T, int P, int U, bool ENT>
+// A lane takes P neighbouring cases of U classes; the cases that fill no pack are taken one a lane (P = 1) by the lanes behind the packs'.
+template <class T, int P, int U, bool ENT, bool NT>
 __global__ void __launch_bounds__(LT) k_log_probs_grad_cols(LogProbGradArgs g, int logG) {
-    const int G = 1 << logG, R = LT >> logG;
-    const int gg = threadIdx.x & (G - 1), r = threadIdx.x >> logG;
-    const int tiles = (g.numCases + G * P - 1) / (G * P);
-    const int n0 = (blockIdx.x % tiles * G + gg) * P;
-    const int j0 = (int)(blockIdx.x / tiles) * (R * U) + r;
-    if (n0 >= g.numCases) return;
-    const T* x = static_cast<const T*>(g.logits) + (size_t)n0 * (P == 1 ? g.caseStride : 1);
-    T* out = static_cast<T*>(g.target) + (size_t)n0 * (P == 1 ? g.targetCaseStride : 1);
-    const bool whole = n0 <= g.numCases - P;
-    Pack<T, P> v[U], t[U];
+    const int G = 1 << logG, R = LT >> logG, packs = g.numCases / P, columns = packs + g.numCases % P;
+    const int tiles = (columns + G - 1) >> logG;
+    const int column = ((int)(blockIdx.x % tiles) << logG) + (threadIdx.x & (G - 1));
+    const int j0 = (int)(blockIdx.x / tiles) * (R * U) + (threadIdx.x >> logG);
+    if (column >= columns || j0 >= g.numOut) return;
+    const T* logits = static_cast<const T*>(g.logits);
+    T* target = static_cast<T*>(g.target);
+    const Pass pass;
+    const auto take = [&](auto width, int n0) {
+        constexpr int N = decltype(width)::value;
+        const T* x = logits + (size_t)n0 * (P == 1 ? g.caseStride : 1);
+        T* out = target + (size_t)n0 * (P == 1 ? g.targetCaseStride : 1);
+        Words<T, N> v[U], t[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const int j = j0 + u * R;
-        if (j >= g.numOut) continue;
-        const T* from = x + (size_t)j * g.classStride;
-        const T* prev = out + (size_t)j * g.targetClassStride;
-        if (whole) {
-            v[u] = load_pack<T, P>(from, g.nt);
-            if (g.add) t[u] = load_pack<T, P>(prev, g.nt);
-        } else {
+        for (int u = 0; u < U; ++u) v[u].template load<NT>(x + (size_t)min(j0 + u * R, g.numOut - 1) * g.classStride);
+        if (g.add) {
 #pragma unroll
-            for (int k = 0; k < P; ++k) {
-                v[u].v[k] = n0 < g.numCases - k ? from[k] : (T)0.f;
-                if (g.add) t[u].v[k] = n0 < g.numCases - k ? prev[k] : (T)0.f;
+            for (int u = 0; u < U; ++u) t[u].template load<NT>(out + (size_t)min(j0 + u * R, g.numOut - 1) * g.targetClassStride);
+        }
+        CaseGrad c[N];
+#pragma unroll
+        for (int k = 0; k < N; ++k) c[k] = case_grad<ENT>(g, n0 + k);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int j = j0 + u * R;
+            if (j >= g.numOut) break;
+            Pack<T, N> d;
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                float y = grad_of<ENT>(v[u].at(k, pass), c[k]) + (j == c[k].y ? c[k].a : 0.f);
+                if (g.add) y += t[u].at(k, pass);
+                d.v[k] = (T)y;
             }
+            store_pack<NT, T, N>(out + (size_t)j * g.targetClassStride, d);
         }
-    }
-    CaseGrad c[P];
-#pragma unroll
-    for (int k = 0; k < P; ++k) c[k] = case_grad<ENT>(g, min(n0 + k, g.numCases - 1));
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const int j = j0 + u * R;
-        if (j >= g.numOut) continue;
-        T* to = out + (size_t)j * g.targetClassStride;
-        Pack<T, P> d;
-#pragma unroll
-        for (int k = 0; k < P; ++k) {
-            float y = grad_of<ENT>((float)v[u].v[k], c[k]) + (j == c[k].y ? c[k].a : 0.f);
-            if (g.add) y += (float)t[u].v[k];
-            d.v[k] = (T)y;
-        }
-        if (whole) store_pack<T, P>(to, d, g.nt);
-        else {
-#pragma unroll
-            for (int k = 0; k < P; ++k)
-                if (n0 < g.numCases - k) to[k] = d.v[k];
-        }
-    }
+    };
+    if (P > 1 && column >= packs) take(std::integral_constant<int, 1>(), packs * P + (column - packs));
+    else take(std::integral_constant<int, P>(), column * P);
 }
 
 // Element (class j, case n) at j*classStride + n*caseStride.  BY_CASE: a case's classes side by side; BY_CLASS: a class's cases.
@@ -877,31 +856,36 @@ Plan plan_log_probs(int type, int kinds, int numCases, int numOut, int numTop) {
     return p;
 }
 
-template <class T, bool ENT, bool TOP>
+template <class T, bool ENT, bool TOP, bool NT>
 void launch_rows(const Plan& p, const LogProbArgs& a, hipStream_t s) {
     const dim3 grid((unsigned)p.blocks), block(LT);
     if (p.threads == 64) {
-        if (p.U == 1) hipLaunchKernelGGL((k_log_probs_rows<T, 64, 1, ENT, TOP>), grid, block, 0, s, a, p.parts);
-        else hipLaunchKernelGGL((k_log_probs_rows<T, 64, 4, ENT, TOP>), grid, block, 0, s, a, p.parts);
-    } else if (p.U == 1) hipLaunchKernelGGL((k_log_probs_rows<T, LT, 1, ENT, TOP>), grid, block, 0, s, a, p.parts);
-    else if (p.U == 4) hipLaunchKernelGGL((k_log_probs_rows<T, LT, 4, ENT, TOP>), grid, block, 0, s, a, p.parts);
-    else hipLaunchKernelGGL((k_log_probs_rows<T, LT, 16, ENT, TOP>), grid, block, 0, s, a, p.parts);
+        if (p.U == 1) hipLaunchKernelGGL((k_log_probs_rows<T, 64, 1, ENT, TOP, NT>), grid, block, 0, s, a, p.parts);
+        else hipLaunchKernelGGL((k_log_probs_rows<T, 64, 4, ENT, TOP, NT>), grid, block, 0, s, a, p.parts);
+    } else if (p.U == 1) hipLaunchKernelGGL((k_log_probs_rows<T, LT, 1, ENT, TOP, false>), grid, block, 0, s, a, p.parts);   // (few cases: little data)
+    else if (p.U == 4) hipLaunchKernelGGL((k_log_probs_rows<T, LT, 4, ENT, TOP, NT>), grid, block, 0, s, a, p.parts);
+    else hipLaunchKernelGGL((k_log_probs_rows<T, LT, 16, ENT, TOP, NT>), grid, block, 0, s, a, p.parts);
 }
-template <class T, int P, bool ENT, bool TOP>
+template <class T, int P, bool ENT, bool TOP, bool NT>
 void launch_cols(const Plan& p, const LogProbArgs& a, hipStream_t s) {
     const dim3 grid((unsigned)p.blocks), block(LT);
     const size_t lds = TOP ? col_lds_bytes(P << p.logG, std::min(p.U, 4) * (LT >> p.logG)) : 0;
-    if (p.U == 1) hipLaunchKernelGGL((k_log_probs_cols<T, P, 1, ENT, TOP>), grid, block, lds, s, a, p.parts, p.logG);
-    else if (p.U == 4) hipLaunchKernelGGL((k_log_probs_cols<T, P, 4, ENT, TOP>), grid, block, lds, s, a, p.parts, p.logG);
-    else hipLaunchKernelGGL((k_log_probs_cols<T, P, 16, ENT, TOP>), grid, block, lds, s, a, p.parts, p.logG);
+    if (p.U == 1) hipLaunchKernelGGL((k_log_probs_cols<T, P, 1, ENT, TOP, NT>), grid, block, lds, s, a, p.parts, p.logG);
+    else if (p.U == 4) hipLaunchKernelGGL((k_log_probs_cols<T, P, 4, ENT, TOP, NT>), grid, block, lds, s, a, p.parts, p.logG);
+    else hipLaunchKernelGGL((k_log_probs_cols<T, P, 16, ENT, TOP, NT>), grid, block, lds, s, a, p.parts, p.logG);
+}
+template <class T, bool ENT, bool TOP, bool NT>
+void launch_parts(const Plan& p, const LogProbArgs& a, hipStream_t s) {
+    if (p.rows) launch_rows<T, ENT, TOP, NT>(p, a, s);
+    else if (p.P == 1) launch_cols<T, 1, ENT, TOP, false>(p, a, s);
+    else launch_cols<T, TOP ? 4 : 16 / (int)sizeof(T), ENT, TOP, NT>(p, a, s);
 }
 template <class T, bool ENT, bool TOP>
 void launch_log_probs(const Plan& p, const LogProbArgs& a, hipStream_t s) {
-    if (p.rows) launch_rows<T, ENT, TOP>(p, a, s);
-    else if (p.P == 1) launch_cols<T, 1, ENT, TOP>(p, a, s);
-    else launch_cols<T, TOP ? 4 : 16 / (int)sizeof(T), ENT, TOP>(p, a, s);
+    if (streams((size_t)a.numCases * a.numOut * sizeof(T))) launch_parts<T, ENT, TOP, true>(p, a, s);
+    else launch_parts<T, ENT, TOP, false>(p, a, s);
     if (p.parts.parts == 1) return;
-    // a wave joins up to 64 parts; few cases of many parts take a workgroup each
+    // a wave joins up to 16 parts; cases of many parts take a workgroup each
     if (p.parts.parts <= 16) hipLaunchKernelGGL((k_log_probs_join<T, 64>), dim3(ceil_div(a.numCases, LT / 64)), dim3(LT), 0, s, a, p.parts);
     else hipLaunchKernelGGL((k_log_probs_join<T, LT>), dim3(a.numCases), dim3(LT), 0, s, a, p.parts);
 }
@@ -919,20 +903,20 @@ void launch_grad_rows(const LogProbGradArgs& g, hipStream_t s) {
         hipLaunchKernelGGL((k_log_probs_grad_rows<T, LT, U, ENT, NT>), dim3((unsigned)((size_t)g.numCases * parts)), block, 0, s, g, parts);
     }
 }
+template <class T, bool ENT, bool NT>
+void launch_grad_cols(const LogProbGradArgs& g, hipStream_t s) {
+    constexpr int V = 16 / (int)sizeof(T), U = 4;
+    const int columns = g.numCases < V ? g.numCases : g.numCases / V + g.numCases % V;
+    int logG = 0;
+    while (logG < 4 && (1 << logG) < columns) ++logG;
+    const dim3 block(LT), grid((unsigned)((size_t)ceil_div(columns, 1 << logG) * ceil_div(g.numOut, (LT >> logG) * U)));
+    if (g.numCases < V) hipLaunchKernelGGL((k_log_probs_grad_cols<T, 1, U, ENT, false>), grid, block, 0, s, g, logG);
+    else hipLaunchKernelGGL((k_log_probs_grad_cols<T, V, U, ENT, NT>), grid, block, 0, s, g, logG);
+}
 template <class T, bool ENT>
 void launch_grad(const LogProbGradArgs& g, bool rows, hipStream_t s) {
-    constexpr int V = 16 / (int)sizeof(T);
-    if (rows) {
-        if (g.nt) launch_grad_rows<T, ENT, true>(g, s);
-        else launch_grad_rows<T, ENT, false>(g, s);
-        return;
-    }
-    int logG = 0;
-    const int P = g.numCases < V ? 1 : V;
-    while (logG < 4 && (P << logG) < g.numCases) ++logG;
-    const dim3 block(LT), grid((unsigned)((size_t)ceil_div(g.numCases, P << logG) * ceil_div(g.numOut, (LT >> logG) * 4)));
-    if (P == 1) hipLaunchKernelGGL((k_log_probs_grad_cols<T, 1, 4, ENT>), grid, block, 0, s, g, logG);
-    else hipLaunchKernelGGL((k_log_probs_grad_cols<T, V, 4, ENT>), grid, block, 0, s, g, logG);
+    if (streams((size_t)g.numCases * g.numOut * sizeof(T) * 2)) rows ? launch_grad_rows<T, ENT, true>(g, s) : launch_grad_cols<T, ENT, true>(g, s);
+    else rows ? launch_grad_rows<T, ENT, false>(g, s) : launch_grad_cols<T, ENT, false>(g, s);
 }
 
 }  // namespace
@@ -973,7 +957,7 @@ int mc_log_probs(const void* logits, int type, long long classStride, long long 
     p.parts.stats = static_cast<Part*>(workspace);
     p.parts.keys = reinterpret_cast<unsigned long long*>(p.parts.stats + (p.bytes ? (size_t)numCases * p.parts.parts : 0));
     const LogProbArgs a{logits, (size_t)classStride, (size_t)caseStride, labels, labelType, numCases, numOut, labelLogProbs, entropy, maxAndLogSum,
-                        topClasses, topLogProbs, numTop, streams((size_t)numCases * numOut * elem_size(type))};
+                        topClasses, topLogProbs, numTop};
     with_type(type, [&](auto t) {
         typedef decltype(t) T;
         if (numTop) launch_log_probs<T, true, true>(p, a, S(s));
@@ -1009,8 +993,7 @@ int mc_log_probs_grad(const void* logits, int type, long long classStride, long 
     MC_REQUIRE(scaleEntropy == 0.f || entropy, "mc_log_probs_grad: the entropy's gradient needs the entropy");
     MC_REQUIRE(stream_on_current_device(s), "mc_log_probs_grad: the stream belongs to another device than the current one");
     const LogProbGradArgs a{logits, (size_t)classStride, (size_t)caseStride, labels, labelType, numCases, numOut, maxAndLogSum, entropy, gradLabel,
-                            gradEntropy, gradLogZ, scaleLabel, scaleEntropy, scaleLogZ, target, (size_t)targetClassStride, (size_t)targetCaseStride, add,
-                            streams((size_t)numCases * numOut * elem_size(type) * 2)};
+                            gradEntropy, gradLogZ, scaleLabel, scaleEntropy, scaleLogZ, target, (size_t)targetClassStride, (size_t)targetCaseStride, add};
     with_type(type, [&](auto t) {
         typedef decltype(t) T;
         if (scaleEntropy != 0.f) launch_grad<T, true>(a, kinds & targetKinds & BY_CASE, S(s));
