@@ -274,6 +274,12 @@ __device__ __forceinline__ float max_in(const Words<T, N>& v, Pass p) {
     for (int i = 1; i < v.COUNT; ++i) asm("v_pk_max_f16 %0, %1, %2" : "=v"(m.w[0]) : "v"(m.w[0]), "v"(v.w[i]));
     return fmaxf(m.at(0, p), m.at(1, p));
 }
+// The larger of two pairs of 16-bit integers, half by half.
+__device__ __forceinline__ unsigned max_pairs(unsigned a, unsigned b) {
+    unsigned r;
+    asm("v_pk_max_i16 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+}
 // Element k as fma(x, scale, -c); a half goes into the fma as it is (volatile: see Pass).
 template <class T, int N>
 __device__ __forceinline__ float shifted(const Words<T, N>& v, int k, Shift h, Pass p) {
@@ -313,14 +319,19 @@ __global__ void __launch_bounds__(LT) __attribute__((amdgpu_waves_per_eu(4))) k_
     Words<T, V> v[U];
     const int first = tid * V, last = len - V, back = max(-last, 0);
     const bool whole = THREADS == LT || a.numOut >= V;
-    if (whole) {
+    if (len == THREADS * U * V) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const T* base = x + u * (THREADS * V);
+            asm("" : "+s"(base));   // the scalar unit's sum, and one offset for all
+            v[u].template load<NT>(base + (unsigned)first);
+        }
+    } else if (whole) {
         const T* from = x - back;
 #pragma unroll
         for (int u = 0; u < U; ++u) v[u].template load<NT>(from + (unsigned)(min(first + u * (THREADS * V), last) + back));
-        if (len != THREADS * U * V) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) v[u].fill_first(first + u * (THREADS * V) - last);
-        }
+        for (int u = 0; u < U; ++u) v[u].fill_first(first + u * (THREADS * V) - last);
     } else {   // fewer classes than a pack holds
 #pragma unroll
         for (int u = 0; u < U; ++u) v[u].fill();
@@ -330,18 +341,41 @@ __global__ void __launch_bounds__(LT) __attribute__((amdgpu_waves_per_eu(4))) k_
     }
     const float labelLogit = label >= 0 ? (float)x[label] : 0.f;   // (one part: lo is 0)
 
-    float pm[U];
-    {
+    // The packs' maxima.  bf16: as pairs of 16-bit integers first, in whose order non-negative numbers are, and below them the negative ones,
+    // backwards; where the group's largest is not negative (nor infinite, nor NaN), it is right, and a pack's is right if it is not negative
+    // and too low otherwise.  Half the instructions of taking the pairs apart.
+    constexpr bool PAIRS = __is_same(T, __bf16);
+    unsigned pw[U];
+    const auto pm = [&](int u) { return __uint_as_float(pw[u]); };
+    const auto find_maxima = [&] {
         const Pass pass;
 #pragma unroll
-        for (int u = 0; u < U; ++u) pm[u] = max_in(v[u], pass);
+        for (int u = 0; u < U; ++u) pw[u] = __float_as_uint(max_in(v[u], pass));
+        return max_of<U>(pm);
+    };
+    float mine = 0.f, m = 0.f;
+    bool pairs = false;
+    if (PAIRS) {
+        unsigned all = 0;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            pw[u] = max_pairs(max_pairs(v[u].w[0], v[u].w[1]), max_pairs(v[u].w[2], v[u].w[3]));
+            all = u ? max_pairs(all, pw[u]) : pw[u];
+        }
+        const int i = max((int)(short)all, (int)all >> 16);
+        mine = i > 0x7f7f ? INFINITY : __int_as_float(i << 16);
+        m = G::max(mine, shRed[group]);
+        pairs = m >= 0.f && m < kHuge;
+        if (!pairs) G::sync();
     }
-    const float mine = max_of<U>([&](int u) { return pm[u]; });
+    if (!pairs) {
+        mine = find_maxima();
+        m = G::max(mine, shRed[group]);
+    }
     if (TOP) {
         shMax[threadIdx.x] = mine;
         if (tid == 0) shCount[group] = shPacks[group] = 0;
     }
-    const float m = G::max(mine, shRed[group]);
     float s, w;
     const Shift h = shift_for(m);
     {
@@ -368,9 +402,15 @@ __global__ void __launch_bounds__(LT) __attribute__((amdgpu_waves_per_eu(4))) k_
 #pragma unroll
     for (int i = 0; i < THREADS / 64; ++i) q[i] = shMax[group * THREADS + i * 64 + (threadIdx.x & 63)];
     const float threshold = len <= kFewClasses ? -INFINITY : top_threshold(q, a.numTop, m, ~0ull);
+    if (pairs && !(threshold > 0.f)) {
+        find_maxima();
+        pairs = false;
+    }
+    // (reaching a positive threshold is, for the pairs, exceeding the bf16 below it)
+    const unsigned under = ((__float_as_uint(threshold) + 0xffffu) >> 16) - 1, below = under << 16 | (under & 0xffffu);
 #pragma unroll
     for (int u = 0; u < U; ++u)
-        if (pm[u] >= threshold && pm[u] > -INFINITY) {
+        if (pairs ? max_pairs(pw[u], below) != below : pm(u) >= threshold && pm(u) > -INFINITY) {
             const int to = atomicAdd(&shPacks[group], 1);
             if (to < PACKS) {
 #pragma unroll
@@ -585,6 +625,7 @@ __global__ void __launch_bounds__(LT) k_log_probs_join(LogProbArgs a, Parts p) {
     if (tid < p.parts) part = stats[tid];
     int label = -1;
     if (a.labelLogProbs) label = label_of(a.labels, a.labelType, n, a.numOut);
+    const unsigned long long tail = a.numTop && tid < p.parts ? keys[(size_t)(tid + 1) * a.numTop - 1] : 0;
     unsigned long long early[EARLY];
 #pragma unroll
     for (int i = 0; i < EARLY; ++i) early[i] = tid + i * THREADS < total ? keys[tid + i * THREADS] : 0;
@@ -618,6 +659,10 @@ __global__ void __launch_bounds__(LT) k_log_probs_join(LogProbArgs a, Parts p) {
 #pragma unroll
         for (int i = 0; i < Q; ++i) q[i] = head[i] ? key_logit(head[i]) : -INFINITY;
         threshold = top_threshold(q, a.numTop, m, ~0ull);
+    } else if (total > kFewClasses / 2) {   // few parts: the last key of any part's list has numTop keys from it up
+        float last = tid < p.parts && tail ? key_logit(tail) : -INFINITY;
+        for (int off = 32; off > 0; off >>= 1) last = fmaxf(last, __shfl_xor(last, off, 64));
+        threshold = last;   // (in the first wave; parts <= numTop are all there, and the others' -inf is a threshold too)
     }
     const auto take = [&](unsigned long long key) {
         if (key && key_logit(key) >= threshold) {
