@@ -27,7 +27,7 @@ struct LogProbArgs {
 };
 
 // What a workgroup leaves of its classes of a case for the joining kernel; its best numTop keys follow in an array of their own.
-struct Part { float m, s, w, pad; };
+struct Part { float m, s, w, label; };   // label: its logit where this part has it, else -inf
 struct Parts {
     Part* stats;                  // (numCases, parts)
     unsigned long long* keys;     // (numCases, parts, numTop), largest first, 0 = none
@@ -35,14 +35,14 @@ struct Parts {
     int span;                     // classes of a part
 };
 
-// The label of case n, or -1 for "no class".
+// The class that a label's 32 bits name, or -1 for "no class".
+__device__ __forceinline__ int label_from(unsigned bits, int labelType, int numOut) {
+    const float f = __uint_as_float(bits);
+    const int y = labelType == MC_I32 ? (int)bits : f >= 0.f && f < (float)numOut ? (int)f : -1;
+    return y >= 0 && y < numOut ? y : -1;
+}
 __device__ __forceinline__ int label_of(const void* labels, int labelType, int n, int numOut) {
-    if (labelType == MC_I32) {
-        const int y = static_cast<const int*>(labels)[n];
-        return y >= 0 && y < numOut ? y : -1;
-    }
-    const float y = static_cast<const float*>(labels)[n];
-    return y >= 0.f && y < (float)numOut ? (int)y : -1;
+    return label_from(static_cast<const unsigned*>(labels)[n], labelType, numOut);
 }
 
 // ---------------------------------------------------------------- groups of threads that share a case
@@ -109,16 +109,32 @@ __device__ __forceinline__ int key_class(unsigned long long key) { return (int)(
 
 constexpr int kCand = 256;   // candidates a group's list holds
 
-// A value that at least k of the group's maxima (v, Q in each of the wave's lanes that `mask` names, the largest of them hi) reach and
-// few more do: at least k classes reach it then, so no class below it is among the best k.  First down from hi in growing steps, then
-// by bisection; ballots count.  Where ties or the step limits stop it early the value is lower than it could be, never too high.
+// The sum of v over `lanes` neighbouring lanes (a power of two), in each of them.
+__device__ __forceinline__ int sum_lanes(int v, int lanes) {
+    v += lanes > 1 ? __builtin_amdgcn_mov_dpp(v, 0xB1, 0xf, 0xf, false) : 0;    // neighbours in pairs,
+    v += lanes > 2 ? __builtin_amdgcn_mov_dpp(v, 0x4E, 0xf, 0xf, false) : 0;    // pairs in fours,
+    v += lanes > 4 ? __builtin_amdgcn_mov_dpp(v, 0x141, 0xf, 0xf, false) : 0;   // fours in eights (mirrored: all four hold the sum),
+    v += lanes > 8 ? __builtin_amdgcn_mov_dpp(v, 0x140, 0xf, 0xf, false) : 0;   // eights in sixteens
+    if (lanes > 16) v += __shfl_xor(v, 16, 64);
+    if (lanes > 32) v += __shfl_xor(v, 32, 64);
+    return v;
+}
+// A value that at least k of a group's maxima (v, Q in each of `lanes` neighbouring lanes, the largest of them hi) reach and few more do:
+// at least k classes reach it then, so no class below it is among the best k.  First down from hi in growing steps, then by bisection.
+// Where ties or the step limits stop it early the value is lower than it could be, never too high.  (Lanes of other groups may be
+// done earlier or later: nothing here reaches beyond a group.)
 template <int Q>
-__device__ __forceinline__ float top_threshold(const float (&v)[Q], int k, float hi, unsigned long long mask) {
+__device__ __forceinline__ float top_threshold(const float (&v)[Q], int k, float hi, int lanes) {
     const auto reach = [&](float y) {
         int count = 0;
+        if (lanes == 64) {   // the scalar unit counts
 #pragma unroll
-        for (int q = 0; q < Q; ++q) count += __popcll(__ballot(v[q] >= y) & mask);
-        return count;
+            for (int q = 0; q < Q; ++q) count += __popcll(__ballot(v[q] >= y));
+            return count;
+        }
+#pragma unroll
+        for (int q = 0; q < Q; ++q) count += v[q] >= y;
+        return sum_lanes(count, lanes);
     };
     if (!(hi > -INFINITY)) return -INFINITY;
     float lo = hi, above = hi, step = fmaxf(1.f, fabsf(hi) * 0x1p-18f);
@@ -173,14 +189,14 @@ __device__ void top_by_scan(const T* x, size_t stride, int from, int to, int k, 
     }
 }
 
-// Orders `count` distinct keys by counting, for each, the larger ones, and gives (rank, key) to `put` for the first k; ranks from
-// count on get key 0.
-template <class F>
+// Orders `count` keys by counting, for each, the larger ones, and gives (rank, key) to `put` for the first k; ranks from count on get
+// key 0.  The keys are distinct, but for zeros where ZEROS says that there may be some.
+template <bool ZEROS, class F>
 __device__ __forceinline__ void rank_keys(const unsigned long long* keys, int count, int k, int tid, int threads, F put) {
     for (int i = tid; i < count; i += threads) {
         const unsigned long long key = keys[i];
         int rank = 0;
-        for (int c = 0; c < count; ++c) rank += keys[c] > key;
+        for (int c = 0; c < count; ++c) rank += keys[c] > key || (ZEROS && key == 0 && c < i && keys[c] == 0);
         if (rank < k) put(rank, key);
     }
     for (int r = count + tid; r < k; r += threads) put(r, 0);
@@ -311,9 +327,6 @@ __global__ void __launch_bounds__(LT) __attribute__((amdgpu_waves_per_eu(4))) k_
     const int n = (int)row, lo = (int)(item - row * p.parts) * p.span;
     const T* x = static_cast<const T*>(a.logits) + row * a.caseStride + lo;   // this part's classes: lo + j, j < len
     const int len = min(a.numOut - lo, p.span);
-    int label = -1;
-    if (p.parts == 1 && a.labelLogProbs) label = label_of(a.labels, a.labelType, n, a.numOut);
-
     // A pack that would reach past the end starts V before the end instead, and what it then repeats of its neighbour becomes -inf.  (A
     // last part shorter than a pack reaches back into the part before it.)
     Words<T, V> v[U];
@@ -339,7 +352,9 @@ __global__ void __launch_bounds__(LT) __attribute__((amdgpu_waves_per_eu(4))) k_
         for (int k = 0; k < V; ++k)
             if (first == 0 && k < len) v[0].set(k, x[k]);
     }
-    const float labelLogit = label >= 0 ? (float)x[label] : 0.f;   // (one part: lo is 0)
+    int label = -1;
+    if (a.labelLogProbs) label = label_of(a.labels, a.labelType, n, a.numOut);
+    const float labelLogit = label >= lo && label < lo + len ? (float)x[label - lo] : -INFINITY;
 
     // The packs' maxima.  bf16: as pairs of 16-bit integers first, in whose order non-negative numbers are, and below them the negative ones,
     // backwards; where the group's largest is not negative (nor infinite, nor NaN), it is right, and a pack's is right if it is not negative
@@ -393,7 +408,7 @@ __global__ void __launch_bounds__(LT) __attribute__((amdgpu_waves_per_eu(4))) k_
     const CaseStats c = case_stats(m, s);
     if (tid == 0) {
         if (p.parts == 1) write_case(a, n, c, s, w, label, labelLogit);
-        else p.stats[item] = {m, s, w, 0.f};
+        else p.stats[item] = {m, s, w, labelLogit};
     }
     if (!TOP) return;
 
@@ -401,7 +416,7 @@ __global__ void __launch_bounds__(LT) __attribute__((amdgpu_waves_per_eu(4))) k_
     float q[THREADS / 64];
 #pragma unroll
     for (int i = 0; i < THREADS / 64; ++i) q[i] = shMax[group * THREADS + i * 64 + (threadIdx.x & 63)];
-    const float threshold = len <= kFewClasses ? -INFINITY : top_threshold(q, a.numTop, m, ~0ull);
+    const float threshold = len <= kFewClasses ? -INFINITY : top_threshold(q, a.numTop, m, 64);
     if (pairs && !(threshold > 0.f)) {
         find_maxima();
         pairs = false;
@@ -436,7 +451,7 @@ __global__ void __launch_bounds__(LT) __attribute__((amdgpu_waves_per_eu(4))) k_
         if (p.parts == 1) write_top(a, n, rank, key, c);
         else p.keys[(size_t)item * a.numTop + rank] = key;
     };
-    if (packs <= PACKS && count <= kCand) rank_keys(shCand[group], count, a.numTop, tid, THREADS, put);
+    if (packs <= PACKS && count <= kCand) rank_keys<false>(shCand[group], count, a.numTop, tid, THREADS, put);
     else {   // ties, or orders that put many of the largest into few packs' reach
         G::sync();
         top_by_scan<THREADS>(x - lo, 1, lo, lo + len, a.numTop, shCand[group] + kCand, shCand[group]);
@@ -447,16 +462,17 @@ __global__ void __launch_bounds__(LT) __attribute__((amdgpu_waves_per_eu(4))) k_
 // ---------------------------------------------------------------- a class's cases side by side
 // A workgroup takes 256 / G classes of G * P cases at a time, U times, into registers: lane (r, g) holds P neighbouring cases of class
 // r of each.  P states a lane are reduced over the lanes that share them, then over the waves.
-constexpr int kColCand = 96;
-// LDS of the top alternatives: the candidate lists (or what top_by_scan needs), the stretches' maxima, the counts, the thresholds
-__host__ __device__ constexpr int col_list_keys(int cases) { return cases * kColCand > LT + MC_MAX_TOP ? cases * kColCand : LT + MC_MAX_TOP; }
-constexpr size_t col_lds_bytes(int cases, int stretches) {
-    return col_list_keys(cases) * sizeof(unsigned long long) + ((size_t)cases * (stretches + 1) + 2 * cases) * sizeof(float);
+// LDS of the top alternatives: the candidate lists (or what top_by_scan needs), the stretches' maxima, the counts, the thresholds.  A list
+// holds what a threshold lets through with room to spare: of s stretches, k of whose maxima reach it, about s ln(s / (s - k)) classes do.
+__host__ __device__ constexpr int col_cand(int top) { return 2 * top + 32; }
+__host__ __device__ constexpr int col_list_keys(int cases, int top) { return cases * col_cand(top) > LT + MC_MAX_TOP ? cases * col_cand(top) : LT + MC_MAX_TOP; }
+constexpr size_t col_lds_bytes(int cases, int stretches, int top) {
+    return col_list_keys(cases, top) * sizeof(unsigned long long) + ((size_t)cases * (stretches + 1) + 2 * cases) * sizeof(float);
 }
 template <class T, int P, int U, bool ENT, bool TOP, bool NT>
 __global__ void __launch_bounds__(LT) k_log_probs_cols(LogProbArgs a, Parts p, int logG) {
-    constexpr int W = U >= 4 ? U / 4 : 1, WINDOWS = U / W;   // the top's maxima are kept for W classes at a time
-    constexpr int Q = P == 1 ? 16 : WINDOWS * P;
+    constexpr int WINDOWS = U >= 2 ? 2 : 1, W = U / WINDOWS;   // the top's maxima are kept for W classes at a time
+    constexpr int Q = P == 1 ? 8 : WINDOWS * P;
     extern __shared__ unsigned long long shDyn[];
     __shared__ float shM[4][8 * P], shS[4][8 * P], shW[4][8 * P];
     const int G = 1 << logG, R = LT >> logG, cases = G * P;
@@ -479,10 +495,10 @@ __global__ void __launch_bounds__(LT) k_log_probs_cols(LogProbArgs a, Parts p, i
     // what the case's own thread will write: its way to memory (the label, then its logit) is begun now
     const int mine = min((int)threadIdx.x, cases - 1), myCase = min((tile * G + mine / P) * P, a.numCases - P) + mine % P;
     int label = -1;
-    float labelLogit = 0.f;
-    if (p.parts == 1 && a.labelLogProbs && (int)threadIdx.x < cases) {
+    float labelLogit = -INFINITY;
+    if (a.labelLogProbs && (int)threadIdx.x < cases) {
         label = label_of(a.labels, a.labelType, myCase, a.numOut);
-        if (label >= 0) labelLogit = (float)static_cast<const T*>(a.logits)[(size_t)label * a.classStride + (size_t)myCase * a.caseStride];
+        if (label >= lo && label < hi) labelLogit = (float)static_cast<const T*>(a.logits)[(size_t)label * a.classStride + (size_t)myCase * a.caseStride];
     }
     float pm[TOP ? WINDOWS : 1][P], m[P], s[P], w[P];
     const Pass first;
@@ -497,7 +513,7 @@ __global__ void __launch_bounds__(LT) k_log_probs_cols(LogProbArgs a, Parts p, i
         }
     }
     // TOP: the maxima of WINDOWS * R stretches for each case, [case][stretch]
-    float* shSeg = reinterpret_cast<float*>(shDyn + col_list_keys(cases));
+    float* shSeg = reinterpret_cast<float*>(shDyn + col_list_keys(cases, a.numTop));
     int* shCount = reinterpret_cast<int*>(shSeg + cases * (WINDOWS * R + 1));
     float* shTau = reinterpret_cast<float*>(shCount + cases);
     if (TOP) {
@@ -547,42 +563,49 @@ __global__ void __launch_bounds__(LT) k_log_probs_cols(LogProbArgs a, Parts p, i
                 shS[0][cc] = c.logSum;   // (these two are read by their own thread only until the next barrier)
                 shW[0][cc] = c.m;
             }
-        } else p.stats[(size_t)n * p.parts + part] = {M, S, Wt, 0.f};
+        } else p.stats[(size_t)n * p.parts + part] = {M, S, Wt, labelLogit};
     }
     if (!TOP) return;
 
-    // thresholds: `lanes` neighbouring lanes share a case's maxima
-    const int lanes = min(64, LT / cases), owner = threadIdx.x / lanes, sub = threadIdx.x % lanes, stretches = WINDOWS * R;
-    {
+    const int lanes = min(64, LT / cases), owner = threadIdx.x / lanes, sub = threadIdx.x % lanes, stretches = WINDOWS * R, cap = col_cand(a.numTop);
+    const int len = hi - lo;
+    const bool few = len <= kFewClasses / 2;   // then each class has a place in its cases' lists
+    const Pass third;
+    if (few) {
+#pragma unroll
+        for (int k = 0; k < P; ++k)
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (u * R + r < len) shDyn[(g * P + k) * cap + u * R + r] = top_key(v[u].at(k, third), lo + u * R + r);
+    } else {
+        // thresholds: `lanes` neighbouring lanes share a case's maxima
         float q[Q];
 #pragma unroll
         for (int i = 0; i < Q; ++i) {
             const int at = sub + i * lanes;
             q[i] = owner < cases && at < stretches ? shSeg[owner * (stretches + 1) + at] : -INFINITY;
         }
-        const unsigned long long mask = (lanes == 64 ? ~0ull : (1ull << lanes) - 1) << (lane - lane % lanes);
         const int own = min(owner, cases - 1);
         const float most = fmaxf(fmaxf(shM[0][own], shM[1][own]), fmaxf(shM[2][own], shM[3][own]));
-        const float tau = hi - lo <= kFewClasses / 2 ? -INFINITY : top_threshold(q, a.numTop, most, mask);
+        const float tau = top_threshold(q, a.numTop, most, lanes);
         if (owner < cases && sub == 0) shTau[owner] = tau;
-    }
-    __syncthreads();
-    const Pass third;
+        __syncthreads();
 #pragma unroll
-    for (int k = 0; k < P; ++k) {
-        const float tau = shTau[g * P + k];
+        for (int k = 0; k < P; ++k) {
+            const float tau = shTau[g * P + k];
 #pragma unroll
-        for (int i = 0; i < WINDOWS; ++i)
-            if (pm[i][k] >= tau) {
+            for (int i = 0; i < WINDOWS; ++i)
+                if (pm[i][k] >= tau) {
 #pragma unroll
-                for (int u = 0; u < W; ++u) {
-                    const float y = v[i * W + u].at(k, third);
-                    if (y >= tau && y > -INFINITY) {
-                        const int to = atomicAdd(&shCount[g * P + k], 1);
-                        if (to < kColCand) shDyn[(g * P + k) * kColCand + to] = top_key(y, lo + (i * W + u) * R + r);
+                    for (int u = 0; u < W; ++u) {
+                        const float y = v[i * W + u].at(k, third);
+                        if (y >= tau && y > -INFINITY) {
+                            const int to = atomicAdd(&shCount[g * P + k], 1);
+                            if (to < cap) shDyn[(g * P + k) * cap + to] = top_key(y, lo + (i * W + u) * R + r);
+                        }
                     }
                 }
-            }
+        }
     }
     __syncthreads();
     const auto put = [&](int cc, int rank, unsigned long long key) {
@@ -590,11 +613,11 @@ __global__ void __launch_bounds__(LT) k_log_probs_cols(LogProbArgs a, Parts p, i
         if (p.parts == 1) write_top(a, n, rank, key, CaseStats{shW[0][cc], shS[0][cc], 0.f});
         else p.keys[((size_t)n * p.parts + part) * a.numTop + rank] = key;
     };
-    if (owner < cases && shCount[owner] <= kColCand)
-        rank_keys(shDyn + owner * kColCand, shCount[owner], a.numTop, sub, lanes, [&](int rank, unsigned long long key) { put(owner, rank, key); });
-    __syncthreads();
+    const int count = owner < cases ? few ? len : shCount[owner] : 0;
+    if (owner < cases && count <= cap) rank_keys<true>(shDyn + owner * cap, count, a.numTop, sub, lanes, [&](int rank, unsigned long long key) { put(owner, rank, key); });
+    if (!__syncthreads_or(count > cap)) return;
     for (int cc = 0; cc < cases; ++cc) {   // lists that overflowed: the lists' memory is free by now
-        if (shCount[cc] <= kColCand) continue;
+        if (shCount[cc] <= cap) continue;
         const int n = min((tile * G + cc / P) * P, a.numCases - P) + cc % P;
         top_by_scan<LT>(static_cast<const T*>(a.logits) + (size_t)n * a.caseStride, a.classStride, lo, hi, a.numTop, shDyn + LT, shDyn);
         if ((int)threadIdx.x < a.numTop) put(cc, threadIdx.x, shDyn[LT + threadIdx.x]);
@@ -604,24 +627,24 @@ __global__ void __launch_bounds__(LT) k_log_probs_cols(LogProbArgs a, Parts p, i
 
 // ---------------------------------------------------------------- joining the parts of a case
 constexpr int kJoinCand = 1024;
-template <class T, int THREADS>
+template <int THREADS>
 __global__ void __launch_bounds__(LT) k_log_probs_join(LogProbArgs a, Parts p) {
     typedef Group<THREADS> G;
     constexpr int GROUPS = LT / THREADS, CAND = THREADS == 64 ? kJoinCand / 4 : kJoinCand;
-    __shared__ float shRed[GROUPS][3 * G::WAVES];
+    __shared__ float shRed[GROUPS][4 * G::WAVES];
     __shared__ unsigned long long shCand[GROUPS][CAND];
     __shared__ int shCount[GROUPS];
     const int group = G::index(), tid = G::tid();
     const size_t row = (size_t)blockIdx.x * GROUPS + group;
     if (row >= (size_t)a.numCases) return;
     const int n = (int)row;
-    // All that is read is under way before anything is waited for: statistics, label (and then its logit), the parts' best keys, and as many
-    // of all keys as the threads hold at EARLY each.
+    // All that is read is under way before anything is waited for: statistics, label, the parts' best keys, and as many of all keys as the
+    // threads hold at EARLY each.
     constexpr int EARLY = 6;
     const Part* stats = p.stats + row * p.parts;
     const unsigned long long* keys = p.keys + row * p.parts * a.numTop;
     const int total = p.parts * a.numTop;
-    Part part = {-INFINITY, 0.f, 0.f, 0.f};
+    Part part = {-INFINITY, 0.f, 0.f, -INFINITY};
     if (tid < p.parts) part = stats[tid];
     int label = -1;
     if (a.labelLogProbs) label = label_of(a.labels, a.labelType, n, a.numOut);
@@ -635,10 +658,12 @@ __global__ void __launch_bounds__(LT) k_log_probs_join(LogProbArgs a, Parts p) {
     const int heads = min(p.parts, 64 * Q);   // (beyond: the first ones' threshold holds too)
 #pragma unroll
     for (int i = 0; i < Q; ++i) head[i] = thresholds && (int)(threadIdx.x & 63) + 64 * i < heads ? keys[(size_t)((threadIdx.x & 63) + 64 * i) * a.numTop] : 0;
-    const float labelLogit = label >= 0 ? (float)static_cast<const T*>(a.logits)[(size_t)label * a.classStride + row * a.caseStride] : 0.f;
     if (tid == 0) shCount[group] = 0;
-    float m = part.m;
-    for (int i = tid + THREADS; i < p.parts; i += THREADS) m = fmaxf(m, stats[i].m);
+    float m = part.m, labelLogit = part.label;
+    for (int i = tid + THREADS; i < p.parts; i += THREADS) {
+        m = fmaxf(m, stats[i].m);
+        labelLogit = fmaxf(labelLogit, stats[i].label);
+    }
     m = G::max(m, shRed[group]);
     float s = 0.f, w = 0.f;
     for (int i = tid; i < p.parts; i += THREADS) {
@@ -648,6 +673,7 @@ __global__ void __launch_bounds__(LT) k_log_probs_join(LogProbArgs a, Parts p) {
         w += fmaf(fmaxf(d, -200.f), part.s, part.w) * f;
     }
     G::sum2(s, w, shRed[group] + G::WAVES);
+    labelLogit = G::max(labelLogit, shRed[group] + 3 * G::WAVES);
     const CaseStats c = case_stats(m, s);
     if (tid == 0) write_case(a, n, c, s, w, label, labelLogit);
     if (!a.numTop) return;
@@ -658,7 +684,7 @@ __global__ void __launch_bounds__(LT) k_log_probs_join(LogProbArgs a, Parts p) {
         float q[Q];
 #pragma unroll
         for (int i = 0; i < Q; ++i) q[i] = head[i] ? key_logit(head[i]) : -INFINITY;
-        threshold = top_threshold(q, a.numTop, m, ~0ull);
+        threshold = top_threshold(q, a.numTop, m, 64);
     } else if (total > kFewClasses / 2) {   // few parts: the last key of any part's list has numTop keys from it up
         float last = tid < p.parts && tail ? key_logit(tail) : -INFINITY;
         for (int off = 32; off > 0; off >>= 1) last = fmaxf(last, __shfl_xor(last, off, 64));
@@ -677,7 +703,7 @@ __global__ void __launch_bounds__(LT) k_log_probs_join(LogProbArgs a, Parts p) {
     G::sync();
     const int count = shCount[group];
     if (count <= CAND) {
-        rank_keys(shCand[group], count, a.numTop, tid, THREADS, [&](int rank, unsigned long long key) { write_top(a, n, rank, key, c); });
+        rank_keys<false>(shCand[group], count, a.numTop, tid, THREADS, [&](int rank, unsigned long long key) { write_top(a, n, rank, key, c); });
         return;
     }
     // more ties than the list holds: the best, then the best below it, and so on
@@ -716,21 +742,48 @@ struct LogProbGradArgs {
 
 // d_j = p_j (A - h (ln p_j + H)) + [j = y] a
 struct CaseGrad { float m, logSum, A, h, H, a; int y; };
+// A case's weights, of N neighbouring cases.
+template <int N>
+__device__ __forceinline__ void load_words(const void* p, int n0, unsigned (&w)[N]) {
+    constexpr int V = N % 4 == 0 ? 4 : 1;
+#pragma unroll
+    for (int i = 0; i < N; i += V) {
+        Words<float, V> q;
+        q.template load<false>(static_cast<const float*>(p) + n0 + i);
+#pragma unroll
+        for (int k = 0; k < V; ++k) w[i + k] = q.w[k];
+    }
+}
+template <bool ENT, int N>
+__device__ __forceinline__ void case_grads(const LogProbGradArgs& g, int n0, CaseGrad (&c)[N]) {
+    unsigned m[N], logSum[N], y[N], gl[N], gz[N], ge[N], H[N];
+    load_words(g.maxAndLogSum, n0, m);
+    load_words(g.maxAndLogSum + g.numCases, n0, logSum);
+    if (g.scaleLabel != 0.f) load_words(g.labels, n0, y);
+    if (g.scaleLabel != 0.f && g.gradLabel) load_words(g.gradLabel, n0, gl);
+    if (g.scaleLogZ != 0.f && g.gradLogZ) load_words(g.gradLogZ, n0, gz);
+    if (ENT && g.gradEntropy) load_words(g.gradEntropy, n0, ge);
+    if (ENT) load_words(g.entropy, n0, H);
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        c[k].m = __uint_as_float(m[k]);
+        c[k].logSum = __uint_as_float(logSum[k]);
+        c[k].y = g.scaleLabel != 0.f ? label_from(y[k], g.labelType, g.numOut) : -1;
+        c[k].a = c[k].y >= 0 ? g.scaleLabel * (g.gradLabel ? __uint_as_float(gl[k]) : 1.f) : 0.f;
+        c[k].A = (g.scaleLogZ != 0.f ? g.scaleLogZ * (g.gradLogZ ? __uint_as_float(gz[k]) : 1.f) : 0.f) - c[k].a;
+        c[k].h = ENT ? g.scaleEntropy * (g.gradEntropy ? __uint_as_float(ge[k]) : 1.f) : 0.f;
+        c[k].H = ENT ? __uint_as_float(H[k]) : 0.f;
+        if (c[k].m == -INFINITY) {   // every class is ruled out: p = 0 throughout, and the label's term goes too
+            c[k].m = c[k].logSum = c[k].a = 0.f;
+            c[k].y = -1;
+        }
+    }
+}
 template <bool ENT>
 __device__ __forceinline__ CaseGrad case_grad(const LogProbGradArgs& g, int n) {
-    CaseGrad c;
-    c.m = g.maxAndLogSum[n];
-    c.logSum = g.maxAndLogSum[(size_t)g.numCases + n];
-    c.y = g.scaleLabel != 0.f ? label_of(g.labels, g.labelType, n, g.numOut) : -1;
-    c.a = c.y >= 0 ? g.scaleLabel * (g.gradLabel ? g.gradLabel[n] : 1.f) : 0.f;
-    c.A = (g.scaleLogZ != 0.f ? g.scaleLogZ * (g.gradLogZ ? g.gradLogZ[n] : 1.f) : 0.f) - c.a;
-    c.h = ENT ? g.scaleEntropy * (g.gradEntropy ? g.gradEntropy[n] : 1.f) : 0.f;
-    c.H = ENT ? g.entropy[n] : 0.f;
-    if (c.m == -INFINITY) {   // every class is ruled out: p = 0 throughout, and the label's term goes too
-        c.m = c.logSum = c.a = 0.f;
-        c.y = -1;
-    }
-    return c;
+    CaseGrad c[1];
+    case_grads<ENT>(g, n, c);
+    return c[0];
 }
 template <bool ENT>
 __device__ __forceinline__ float grad_of(float x, const CaseGrad& c) {
@@ -790,43 +843,49 @@ __global__ void __launch_bounds__(LT) k_log_probs_grad_rows(LogProbGradArgs g, i
     }
 }
 
-// A lane takes P neighbouring cases of U classes; the cases that fill no pack are taken one a lane (P = 1) by the lanes behind the packs'.
+// A lane takes P neighbouring cases of `rounds` times U classes; the cases that fill no pack are taken one a lane (P = 1) by the lanes
+// behind the packs'.  What a case needs is loaded once for all of a lane's classes.
 template <class T, int P, int U, bool ENT, bool NT>
-__global__ void __launch_bounds__(LT) k_log_probs_grad_cols(LogProbGradArgs g, int logG) {
+__global__ void __launch_bounds__(LT) k_log_probs_grad_cols(LogProbGradArgs g, int logG, int rounds) {
     const int G = 1 << logG, R = LT >> logG, packs = g.numCases / P, columns = packs + g.numCases % P;
     const int tiles = (columns + G - 1) >> logG;
     const int column = ((int)(blockIdx.x % tiles) << logG) + (threadIdx.x & (G - 1));
-    const int j0 = (int)(blockIdx.x / tiles) * (R * U) + (threadIdx.x >> logG);
-    if (column >= columns || j0 >= g.numOut) return;
+    const int from = (int)(blockIdx.x / tiles) * (R * U * rounds) + (threadIdx.x >> logG), to = min(from + R * U * rounds, g.numOut);
+    if (column >= columns) return;
     const T* logits = static_cast<const T*>(g.logits);
     T* target = static_cast<T*>(g.target);
-    const Pass pass;
     const auto take = [&](auto width, int n0) {
         constexpr int N = decltype(width)::value;
         const T* x = logits + (size_t)n0 * (P == 1 ? g.caseStride : 1);
         T* out = target + (size_t)n0 * (P == 1 ? g.targetCaseStride : 1);
-        Words<T, N> v[U], t[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) v[u].template load<NT>(x + (size_t)min(j0 + u * R, g.numOut - 1) * g.classStride);
-        if (g.add) {
-#pragma unroll
-            for (int u = 0; u < U; ++u) t[u].template load<NT>(out + (size_t)min(j0 + u * R, g.numOut - 1) * g.targetClassStride);
-        }
         CaseGrad c[N];
+        case_grads<ENT>(g, n0, c);
+        for (int j0 = from; j0 < to; j0 += R * U) {
+            Words<T, N> v[U];
 #pragma unroll
-        for (int k = 0; k < N; ++k) c[k] = case_grad<ENT>(g, n0 + k);
+            for (int u = 0; u < U; ++u) v[u].template load<NT>(x + (size_t)min(j0 + u * R, g.numOut - 1) * g.classStride);
+            bool here = false;   // is a label of these cases among these classes, or between them?
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int j = j0 + u * R;
-            if (j >= g.numOut) break;
-            Pack<T, N> d;
+            for (int k = 0; k < N; ++k) here |= (unsigned)(c[k].y - j0) < (unsigned)(R * U);
+            const Pass pass;
 #pragma unroll
-            for (int k = 0; k < N; ++k) {
-                float y = grad_of<ENT>(v[u].at(k, pass), c[k]) + (j == c[k].y ? c[k].a : 0.f);
-                if (g.add) y += t[u].at(k, pass);
-                d.v[k] = (T)y;
+            for (int u = 0; u < U; ++u) {
+                const int j = j0 + u * R;
+                Words<T, N> t;
+                if (g.add) t.template load<NT>(out + (size_t)min(j, g.numOut - 1) * g.targetClassStride);
+                Pack<T, N> d;
+                float e[N];
+#pragma unroll
+                for (int k = 0; k < N; ++k) e[k] = grad_of<ENT>(v[u].at(k, pass), c[k]);
+                if (here) {
+#pragma unroll
+                    for (int k = 0; k < N; ++k)
+                        if (j == c[k].y) e[k] += c[k].a;
+                }
+#pragma unroll
+                for (int k = 0; k < N; ++k) d.v[k] = (T)(g.add ? e[k] + t.at(k, pass) : e[k]);
+                if (j < to) store_pack<NT, T, N>(out + (size_t)j * g.targetClassStride, d);
             }
-            store_pack<NT, T, N>(out + (size_t)j * g.targetClassStride, d);
         }
     };
     if (P > 1 && column >= packs) take(std::integral_constant<int, 1>(), packs * P + (column - packs));
@@ -876,23 +935,24 @@ Plan plan_log_probs(int type, int kinds, int numCases, int numOut, int numTop) {
             p.blocks = ceil_div(numCases, LT / 64);
         } else {
             p.threads = LT;
-            for (p.U = 16; p.U > 1 && (size_t)numCases * ceil_div(numOut, LT * V * p.U) < (p.U == 16 ? 4 : 1) * (size_t)cus; p.U /= 4) {}
+            for (p.U = 16; p.U > 1 && (numOut <= LT * V * (p.U / 4) || (size_t)numCases * ceil_div(numOut, LT * V * p.U) < (p.U == 16 ? 4 : 1) * (size_t)cus); p.U /= 4) {}
             p.parts.parts = ceil_div(numOut, LT * V * p.U);
             p.parts.span = ceil_div(ceil_div(numOut, p.parts.parts), V) * V;
             p.parts.parts = ceil_div(numOut, p.parts.span);
             p.blocks = (size_t)numCases * p.parts.parts;
         }
     } else {
-        p.P = numTop ? 4 : V;
+        p.P = V;
         if (numCases < p.P) p.P = 1;
         // A small matrix: every case in one part, if a workgroup of R classes by 1 ... 16 can hold it.  (Its lines are then read in short
         // pieces, which the L2 makes up for; joining costs a launch.)
         const bool small = (size_t)numCases * numOut * elem_size(type) <= (4u << 20) && numOut <= LT * 16;
+        const int most = numTop && p.P == 8 ? 2 : 3;   // (32 cases' candidates to a workgroup, of 64 classes at a time)
         for (p.U = small ? 1 : 16; small && LT * p.U < numOut; p.U *= 4) {}
-        while (p.logG < 3 && (p.P << p.logG) < numCases && (!small || (LT >> (p.logG + 1)) * p.U >= numOut)) ++p.logG;
+        while (p.logG < most && (p.P << p.logG) < numCases && (!small || (LT >> (p.logG + 1)) * p.U >= numOut)) ++p.logG;
         const int R = LT >> p.logG, tiles = ceil_div(numCases, p.P << p.logG);
-        if (!small)
-            for (; p.U > 1 && (numOut <= R * (p.U / 4) || (size_t)tiles * ceil_div(numOut, R * p.U) < 2 * (size_t)cus); p.U /= 4) {}
+        if (!small)   // (up to 128 parts, or joining them takes longer than what it gains)
+            for (; p.U > 1 && (numOut <= R * (p.U / 4) || ((size_t)tiles * ceil_div(numOut, R * p.U) < 2 * (size_t)cus && ceil_div(numOut, R * (p.U / 4)) <= 128)); p.U /= 4) {}
         p.parts.span = R * p.U;
         p.parts.parts = ceil_div(numOut, p.parts.span);
         p.blocks = (size_t)tiles * p.parts.parts;
@@ -914,7 +974,7 @@ void launch_rows(const Plan& p, const LogProbArgs& a, hipStream_t s) {
 template <class T, int P, bool ENT, bool TOP, bool NT>
 void launch_cols(const Plan& p, const LogProbArgs& a, hipStream_t s) {
     const dim3 grid((unsigned)p.blocks), block(LT);
-    const size_t lds = TOP ? col_lds_bytes(P << p.logG, std::min(p.U, 4) * (LT >> p.logG)) : 0;
+    const size_t lds = TOP ? col_lds_bytes(P << p.logG, std::min(p.U, 2) * (LT >> p.logG), a.numTop) : 0;
     if (p.U == 1) hipLaunchKernelGGL((k_log_probs_cols<T, P, 1, ENT, TOP, NT>), grid, block, lds, s, a, p.parts, p.logG);
     else if (p.U == 4) hipLaunchKernelGGL((k_log_probs_cols<T, P, 4, ENT, TOP, NT>), grid, block, lds, s, a, p.parts, p.logG);
     else hipLaunchKernelGGL((k_log_probs_cols<T, P, 16, ENT, TOP, NT>), grid, block, lds, s, a, p.parts, p.logG);
@@ -923,7 +983,7 @@ template <class T, bool ENT, bool TOP, bool NT>
 void launch_parts(const Plan& p, const LogProbArgs& a, hipStream_t s) {
     if (p.rows) launch_rows<T, ENT, TOP, NT>(p, a, s);
     else if (p.P == 1) launch_cols<T, 1, ENT, TOP, false>(p, a, s);
-    else launch_cols<T, TOP ? 4 : 16 / (int)sizeof(T), ENT, TOP, NT>(p, a, s);
+    else launch_cols<T, 16 / (int)sizeof(T), ENT, TOP, NT>(p, a, s);
 }
 template <class T, bool ENT, bool TOP>
 void launch_log_probs(const Plan& p, const LogProbArgs& a, hipStream_t s) {
@@ -931,8 +991,8 @@ void launch_log_probs(const Plan& p, const LogProbArgs& a, hipStream_t s) {
     else launch_parts<T, ENT, TOP, false>(p, a, s);
     if (p.parts.parts == 1) return;
     // a wave joins up to 16 parts; cases of many parts take a workgroup each
-    if (p.parts.parts <= 16) hipLaunchKernelGGL((k_log_probs_join<T, 64>), dim3(ceil_div(a.numCases, LT / 64)), dim3(LT), 0, s, a, p.parts);
-    else hipLaunchKernelGGL((k_log_probs_join<T, LT>), dim3(a.numCases), dim3(LT), 0, s, a, p.parts);
+    if (p.parts.parts <= 16) hipLaunchKernelGGL((k_log_probs_join<64>), dim3(ceil_div(a.numCases, LT / 64)), dim3(LT), 0, s, a, p.parts);
+    else hipLaunchKernelGGL((k_log_probs_join<LT>), dim3(a.numCases), dim3(LT), 0, s, a, p.parts);
 }
 
 template <class T, bool ENT, bool NT>
@@ -952,11 +1012,13 @@ template <class T, bool ENT, bool NT>
 void launch_grad_cols(const LogProbGradArgs& g, hipStream_t s) {
     constexpr int V = 16 / (int)sizeof(T), U = 4;
     const int columns = g.numCases < V ? g.numCases : g.numCases / V + g.numCases % V;
-    int logG = 0;
+    int logG = 0, rounds = 16;   // (blocks of many rounds, and four of them for each CU)
     while (logG < 4 && (1 << logG) < columns) ++logG;
-    const dim3 block(LT), grid((unsigned)((size_t)ceil_div(columns, 1 << logG) * ceil_div(g.numOut, (LT >> logG) * U)));
-    if (g.numCases < V) hipLaunchKernelGGL((k_log_probs_grad_cols<T, 1, U, ENT, false>), grid, block, 0, s, g, logG);
-    else hipLaunchKernelGGL((k_log_probs_grad_cols<T, V, U, ENT, NT>), grid, block, 0, s, g, logG);
+    const size_t tiles = ceil_div(columns, 1 << logG);
+    while (rounds > 1 && tiles * ceil_div(g.numOut, (LT >> logG) * U * rounds) < 4 * (size_t)num_cus()) rounds /= 2;
+    const dim3 block(LT), grid((unsigned)(tiles * ceil_div(g.numOut, (LT >> logG) * U * rounds)));
+    if (g.numCases < V) hipLaunchKernelGGL((k_log_probs_grad_cols<T, 1, U, ENT, false>), grid, block, 0, s, g, logG, rounds);
+    else hipLaunchKernelGGL((k_log_probs_grad_cols<T, V, U, ENT, NT>), grid, block, 0, s, g, logG, rounds);
 }
 template <class T, bool ENT>
 void launch_grad(const LogProbGradArgs& g, bool rows, hipStream_t s) {
