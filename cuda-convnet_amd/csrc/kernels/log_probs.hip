@@ -45,6 +45,24 @@ __device__ __forceinline__ int label_of(const void* labels, int labelType, int n
     return label_from(static_cast<const unsigned*>(labels)[n], labelType, numOut);
 }
 
+// op over the lanes of a wave whose numbers agree modulo G (1, 2, 4 or 8), in each of them.  Rotations within rows of 16 lanes and swaps
+// of rows: a dozen cycles a step, where a shuffle through the LDS takes a hundred.
+template <int CTRL>
+__device__ __forceinline__ float rotated(float v) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true)); }
+template <class OP>
+__device__ __forceinline__ float over_lanes(float v, int G, OP op) {
+    v = op(v, rotated<0x128>(v));               // by 8,
+    if (G <= 4) v = op(v, rotated<0x124>(v));   // by 4, ...
+    if (G <= 2) v = op(v, rotated<0x122>(v));
+    if (G <= 1) v = op(v, rotated<0x121>(v));
+    const auto rows = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = op(__uint_as_float(rows[0]), __uint_as_float(rows[1]));
+    const auto halves = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return op(__uint_as_float(halves[0]), __uint_as_float(halves[1]));
+}
+struct Larger { __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); } };
+struct Sum { __device__ __forceinline__ float operator()(float a, float b) const { return a + b; } };
+
 // ---------------------------------------------------------------- groups of threads that share a case
 // A whole workgroup, or one wave of it (whose LDS accesses are in order: there only the compiler has to be held back).
 template <int THREADS>
@@ -63,7 +81,7 @@ struct Group {
     __device__ static bool any(bool v) { return THREADS == LT ? __syncthreads_or(v) : __any(v); }
     // sh: WAVES floats of LDS that nobody else uses until the next sync
     __device__ static float max(float v, float* sh) {
-        for (int off = 32; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
+        v = over_lanes(v, 1, Larger());
         if (WAVES == 1) return v;
         if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
         sync();
@@ -73,10 +91,8 @@ struct Group {
         return v;
     }
     __device__ static void sum2(float& a, float& b, float* sh) {
-        for (int off = 32; off > 0; off >>= 1) {
-            a += __shfl_xor(a, off, 64);
-            b += __shfl_xor(b, off, 64);
-        }
+        a = over_lanes(a, 1, Sum());
+        b = over_lanes(b, 1, Sum());
         if (WAVES == 1) return;
         if ((threadIdx.x & 63) == 0) {
             sh[threadIdx.x >> 6] = a;
@@ -525,7 +541,7 @@ __global__ void __launch_bounds__(LT) k_log_probs_cols(LogProbArgs a, Parts p, i
     }
 #pragma unroll
     for (int k = 0; k < P; ++k) {
-        for (int off = 32; off >= G; off >>= 1) m[k] = fmaxf(m[k], __shfl_xor(m[k], off, 64));
+        m[k] = over_lanes(m[k], G, Larger());
         if (lane < G) shM[wave][g * P + k] = m[k];
     }
     __syncthreads();
@@ -541,10 +557,8 @@ __global__ void __launch_bounds__(LT) k_log_probs_cols(LogProbArgs a, Parts p, i
             const Pass pass;
             w[k] = guarded<U>([&](int i) { return fmaf(v[i].at(k, pass), again.scale, -again.c); });
         }
-        for (int off = 32; off >= G; off >>= 1) {
-            s[k] += __shfl_xor(s[k], off, 64);
-            if (ENT) w[k] += __shfl_xor(w[k], off, 64);
-        }
+        s[k] = over_lanes(s[k], G, Sum());
+        if (ENT) w[k] = over_lanes(w[k], G, Sum());
         if (lane < G) {
             shS[wave][g * P + k] = s[k];
             shW[wave][g * P + k] = w[k];
@@ -687,8 +701,7 @@ __global__ void __launch_bounds__(LT) k_log_probs_join(LogProbArgs a, Parts p) {
         threshold = top_threshold(q, a.numTop, m, 64);
     } else if (total > kFewClasses / 2) {   // few parts: the last key of any part's list has numTop keys from it up
         float last = tid < p.parts && tail ? key_logit(tail) : -INFINITY;
-        for (int off = 32; off > 0; off >>= 1) last = fmaxf(last, __shfl_xor(last, off, 64));
-        threshold = last;   // (in the first wave; parts <= numTop are all there, and the others' -inf is a threshold too)
+        threshold = over_lanes(last, 1, Larger());   // (in the first wave; parts <= numTop are all there, and the others' -inf is a threshold too)
     }
     const auto take = [&](unsigned long long key) {
         if (key && key_logit(key) >= threshold) {
