@@ -19,7 +19,7 @@ import dp
 import layer as lay
 from data import DataProvider, DataProviderException
 from gpumodel import IGPUModel, ModelStateException
-from options import BooleanOptionParser, IntegerOptionParser, ListOptionParser, StringOptionParser
+from options import BooleanOptionParser, FloatOptionParser, IntegerOptionParser, ListOptionParser, StringOptionParser
 from util import is_windows_machine
 
 BAR = "-------------------------------------------------------"
@@ -36,6 +36,7 @@ CONVNET_OPTIONS = [
     ("conv-to-local", "conv_to_local", ListOptionParser(StringOptionParser), "Convert given conv layers to unshared local", dict(default=[])),
     ("unshare-weights", "unshare_weights", ListOptionParser(StringOptionParser), "Unshare weight matrices in given layers", dict(default=[])),
     ("conserve-mem", "conserve_mem", BooleanOptionParser, "Conserve GPU memory (slower)?", dict(default=0)),
+    ("clip-norm", "clip_norm", FloatOptionParser, "Largest global norm of a step's gradients (0: no clipping)", dict(default=0.0)),
 ]
 CHANGED_DEFAULTS = {"max_filesize_mb": 0, "testing_freq": 50, "num_epochs": 50000, "dp_type": None}
 CONVNET_PROVIDERS = [
@@ -90,6 +91,8 @@ class ConvNet(IGPUModel):
         self.libmodel.setSeed(base_seed() + self.rank)
         if self.world > 1:
             dp.connect(self.libmodel, self.rank, self.world)
+        if self.op.get_value("clip_norm"):
+            self.libmodel.setGradClip(self.op.get_value("clip_norm"))
 
     def init_model_state(self):
         state = self.model_state

@@ -580,7 +580,62 @@ void ConvNet::buildUpdateSpans() {
     }
 }
 
+// The same tensors as buildUpdateSpans.  The arena holds gradients times their tensor's learning rate (and with the sign of a
+// descent step); the norm is of the gradients themselves, so 1 / eps goes in as the scale.  A tensor that layers share counts with its
+// owner's rate.
+void ConvNet::buildGradSpans() {
+    std::vector<mcGradTensor> tensors;
+    for (Weights* w : _allWeights) {
+        if (w->getEps() <= 0) continue;
+        mcGradTensor t = {};
+        t.grad = w->getGrad();
+        t.count = w->numel();
+        t.scale = 1.f / w->getEps();
+        t.gradType = t.outType = MC_F32;
+        tensors.push_back(t);
+    }
+    int n = 0;
+    RT_MC(mc_grad_spans(tensors.data(), (int)tensors.size(), nullptr, 0, &n));
+    std::vector<mcGradSpan> spans(n);
+    RT_MC(mc_grad_spans(tensors.data(), (int)tensors.size(), spans.data(), n, &n));
+    const size_t bytes = mc_grad_norm_workspace_bytes(n);
+    if (n) {
+        RT_HIP(hipMalloc(reinterpret_cast<void**>(&_gradSpans), n * sizeof(mcGradSpan)));
+        RT_HIP(hipMemcpy(_gradSpans, spans.data(), n * sizeof(mcGradSpan), hipMemcpyHostToDevice));
+    }
+    RT_HIP(hipMalloc(&_normWorkspace, bytes));
+    _normWorkspaceBytes = bytes;
+    const float none[2] = {0.f, 1.f};
+    RT_HIP(hipMalloc(reinterpret_cast<void**>(&_normAndFactor), sizeof(none)));   // last: it tells that the others are there
+    RT_HIP(hipMemcpy(_normAndFactor, none, sizeof(none), hipMemcpyHostToDevice));
+    _numGradSpans = n;
+}
+
+void ConvNet::setGradClip(float maxNorm) {
+    if (!(maxNorm >= 0.f)) throw std::runtime_error("the largest gradient norm must be positive, or 0 for no clipping");
+    if (maxNorm == _clipNorm) return;
+    if (maxNorm > 0.f && !_normAndFactor) buildGradSpans();
+    _clipNorm = maxNorm;
+    DeviceAllocator::get().noteForeignAllocation();   // captured steps hold the launches of the setting they were captured under
+}
+
+void ConvNet::lastGradNorm(float* normAndFactor) {
+    if (_clipNorm <= 0.f) throw std::runtime_error("no gradient norm is taken (setGradClip)");
+    RT_HIP(hipStreamSynchronize(_stream));
+    RT_HIP(hipMemcpy(normAndFactor, _normAndFactor, 2 * sizeof(float), hipMemcpyDeviceToHost));
+}
+
 void ConvNet::updateWeights() {
+    if (_numSpans && _clipNorm > 0.f) {
+        // every rank of a data-parallel group holds the same reduced gradients here and takes the same norm from them: the sums
+        // run in a fixed order, so all ranks scale alike without another exchange
+        profileSetLayer("net");
+        profileSetPhase("update");
+        RT_MC(mc_grad_norm(_gradSpans, _numGradSpans, _clipNorm, _normAndFactor, _normWorkspace, _normWorkspaceBytes, ST()));
+        RT_MC(mc_weights_update_spans_clipped(_arenaW, _arenaInc, _arenaGrad, _spans, _numSpans, _normAndFactor, ST()));
+        for (Weights* w : _allWeights) w->markUpdated();
+        return;
+    }
     if (_numSpans) {
         profileSetLayer("net");
         profileSetPhase("update");
@@ -1052,6 +1107,60 @@ void FeatureWorker::run() {
         float* dst = _ftrs->data() + (size_t)i * dp.getMinibatchSize() * _ftrs->cols();
         for (int c = 0; c < n; c++)
             for (int f = 0; f < acts.rows(); f++) dst[(size_t)c * acts.rows() + f] = host[(size_t)f * n + c];
+    }
+    Cost* cost = _convNet->collectCosts();
+    dp.clearData();
+    _convNet->getResultQueue().enqueue(new WorkResult(WorkResult::BATCH_DONE, cost));
+}
+
+void ConvNet::predict(Layer& logits, DevMat& labels, int numTop, float* out) {
+    DevMat& x = logits.getActs();   // (classes, cases)
+    const int n = x.cols(), cols = 2 + 2 * numTop;
+    _predictions.resize(cols, n);
+    float* p = _predictions.data();
+    int* classes = numTop ? reinterpret_cast<int*>(p + 2 * (size_t)n) : nullptr;
+    const size_t wsb = mc_log_probs_workspace_bytes(MC_F32, n, 1, n, x.rows(), numTop);
+    RT_MC(mc_log_probs(x.data(), MC_F32, n, 1, labels.data(), MC_F32, n, x.rows(), p, p + n, nullptr, classes,
+                       numTop ? p + (size_t)(2 + numTop) * n : nullptr, numTop, wsb ? workspace(wsb) : nullptr, wsb, ST()));
+    std::vector<float> host(_predictions.numel());
+    _predictions.copyToHost(host.data());
+    for (int r = 0; r < cols; r++)
+        for (int c = 0; c < n; c++) {
+            const float v = host[(size_t)r * n + c];
+            int k;
+            memcpy(&k, &v, sizeof(k));
+            out[(size_t)c * cols + r] = r >= 2 && r < 2 + numTop ? (float)k : v;
+        }
+}
+
+void PredictWorker::releaseHost() {
+    DataWorker::releaseHost();
+    if (_out) {
+        _out->release();
+        delete _out;
+        _out = nullptr;
+    }
+}
+
+void PredictWorker::run() {
+    DataProvider& dp = _convNet->getDataProvider();
+    Layer* layer = &_convNet->getLayer(_layerIdx);
+    if (layer->getType() == "softmax") layer = layer->getPrev()[0];
+    const HostMat& labels = *(*_data)[1];   // one row: either order of storage is the same
+    if (labels.rows() != 1) throw std::runtime_error("predictions need one row of labels as the second data matrix");
+    for (size_t i = 0; i < labels.numel(); i++)   // (the cost layers of the pass index the probabilities with them)
+        if (!(labels.data()[i] >= 0 && labels.data()[i] < layer->getNumOutputs()))
+            throw std::runtime_error(fmt("label %g of case %ld is no class of layer '%s'", labels.data()[i], (long)i, layer->getName().c_str()));
+    dp.setData(*_data);
+    if (_out->fortran() || _out->rows() != dp.getNumCases() || _out->cols() != 2 + 2 * _numTop)
+        throw std::runtime_error("prediction matrix must be C-ordered (numCases, 2 + 2 * numTop)");
+    if (layer->getNumOutputs() > 1 << 24) throw std::runtime_error("class numbers above 2^24 do not fit a float32 matrix");
+    _convNet->beginBatchCosts();
+    for (int i = 0; i < dp.getNumMinibatches(); i++) {
+        DevMatV& mini = dp.getMinibatch(i);
+        _convNet->fprop(mini, PASS_TEST);
+        _convNet->endMinibatchCosts(dp.getNumCasesInMinibatch(i));
+        _convNet->predict(*layer, *mini[1], _numTop, _out->data() + (size_t)i * dp.getMinibatchSize() * _out->cols());
     }
     Cost* cost = _convNet->collectCosts();
     dp.clearData();

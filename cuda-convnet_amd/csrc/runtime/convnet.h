@@ -144,6 +144,11 @@ public:
     void copyToCPU();
     void copyToGPU();
     void updateWeights();
+    // gradient clipping: maxNorm > 0 bounds the global norm of every step's gradients (INFINITY only measures it), 0 turns it off
+    void setGradClip(float maxNorm);
+    void lastGradNorm(float* normAndFactor);   // synchronous: norm and factor of the last update under setGradClip
+    // test-mode predictions of a layer's outputs (as logits): out, on the host, is (cases, 2 + 2 * numTop), see PredictWorker
+    void predict(Layer& logits, DevMat& labels, int numTop, float* out);
     void reset();
     void fprop(PASS_TYPE passType);
     void fprop(int miniIdx, PASS_TYPE passType);
@@ -219,6 +224,7 @@ private:
     void initDevice();
     Layer* initLayer(const std::string& layerType, PyObject* paramsDict);
     void buildUpdateSpans();
+    void buildGradSpans();
 
     std::vector<Layer*> _layers;
     std::vector<DataLayer*> _dataLayers;
@@ -237,6 +243,13 @@ private:
     BucketPlanner _buckets;                // which slices of the gradient arena are reduced when (buckets.h)
     mcUpdateSpan* _spans = nullptr;
     int _numSpans = 0;
+    mcGradSpan* _gradSpans = nullptr;      // of the gradients that buildUpdateSpans' spans update; built by the first setGradClip
+    int _numGradSpans = 0;
+    float _clipNorm = 0.f;                 // 0: off
+    float* _normAndFactor = nullptr;
+    void* _normWorkspace = nullptr;
+    size_t _normWorkspaceBytes = 0;
+    DevMat _predictions;                   // kept between calls: a new matrix would drop the captured steps
     float* _workspace = nullptr;
     size_t _workspaceBytes = 0;
     hipStream_t _branchStream = nullptr;   // the weight-gradient branch of a step
@@ -336,6 +349,20 @@ public:
 private:
     HostMat* _ftrs;
     int _layerIdx;
+};
+
+// Test-mode predictions, one row per case: log probability of the case's label, entropy in nats, the
+// numTop likeliest classes (-1 where there are fewer), their log probabilities.  For a softmax layer its input holds the logits.
+class PredictWorker : public DataWorker {
+public:
+    PredictWorker(ConvNet& net, HostMatV* data, HostMat* out, int layerIdx, int numTop)
+        : DataWorker(net, data), _out(out), _layerIdx(layerIdx), _numTop(numTop) {}
+    void run() override;
+    void releaseHost() override;
+
+private:
+    HostMat* _out;
+    int _layerIdx, _numTop;
 };
 
 // Runs `fn` on the device thread and waits for it (used by the extra, non-reference entry

@@ -149,6 +149,27 @@ static PyObject* startFeatureWriter(PyObject*, PyObject* args) {
     return Py_BuildValue("i", 0);
 }
 
+// startPredictions([data, labels, ..., out], layerIdx, numTop): test pass; row n of `out`, C-ordered (cases, 2 + 2 * numTop) float32,
+// receives for case n the log probability of its label, the entropy, the numTop likeliest classes and their log probabilities,
+// with layer layerIdx's outputs (a softmax layer's inputs) as the logits.  Every label is a class.  finishBatch collects it like any batch.
+static PyObject* startPredictions(PyObject*, PyObject* args) {
+    REQUIRE_MODEL();
+    PyObject* data;
+    int layerIdx, numTop;
+    if (!PyArg_ParseTuple(args, "O!ii", &PyList_Type, &data, &layerIdx, &numTop)) return nullptr;
+    if (layerIdx < 0 || layerIdx >= model->getNumLayers() || PyList_GET_SIZE(data) < 3 || numTop < 0 || numTop > MC_MAX_TOP) {
+        PyErr_SetString(PyExc_ValueError, "bad layerIdx / numTop / data list");
+        return nullptr;
+    }
+    try {
+        HostMatV* mvec = getMatrixV(data);
+        HostMat* out = mvec->back();
+        mvec->pop_back();
+        submit(new PredictWorker(*model, mvec, out, layerIdx, numTop));
+    } catch (std::exception& e) { return fail(e); }
+    return Py_BuildValue("i", 0);
+}
+
 static PyObject* finishBatch(PyObject*, PyObject*) {
     REQUIRE_MODEL();
     if (pending.empty()) {
@@ -274,6 +295,30 @@ static PyObject* setSeed(PyObject*, PyObject* args) {
     return Py_BuildValue("i", 0);
 }
 
+// setGradClip(maxNorm): from the next training step on the gradients of all weights are scaled by min(1, maxNorm / norm), norm being
+// their global 2-norm (learning rates not counted); a step whose norm is not finite is dropped.  0 turns it off, inf only measures.
+// Under data parallelism every rank sets the same value.
+static PyObject* setGradClip(PyObject*, PyObject* args) {
+    REQUIRE_MODEL();
+    float maxNorm;
+    if (!PyArg_ParseTuple(args, "f", &maxNorm)) return nullptr;
+    if (!(maxNorm >= 0)) {
+        PyErr_SetString(PyExc_ValueError, "maxNorm must be positive, or 0 for no clipping");
+        return nullptr;
+    }
+    return run_on_device([=] { model->setGradClip(maxNorm); });
+}
+
+// getGradNorm() -> (norm, factor) of the last training step under setGradClip
+static PyObject* getGradNorm(PyObject*, PyObject*) {
+    REQUIRE_MODEL();
+    float nf[2] = {0, 0};
+    PyObject* ok = run_on_device([&] { model->lastGradNorm(nf); });
+    if (!ok) return nullptr;
+    Py_DECREF(ok);
+    return Py_BuildValue("(ff)", nf[0], nf[1]);
+}
+
 // getActs(layerName, grad=0) -> float32 ndarray (outputs, numCases): a layer's current output
 // (or activity gradient); for tests and debugging
 static PyObject* getActs(PyObject*, PyObject* args) {
@@ -360,12 +405,15 @@ static PyMethodDef methods[] = {{"initModel", initModel, METH_VARARGS, nullptr},
                                 {"checkGradients", checkGradients, METH_VARARGS, nullptr},
                                 {"startMultiviewTest", startMultiviewTest, METH_VARARGS, nullptr},
                                 {"startFeatureWriter", startFeatureWriter, METH_VARARGS, nullptr},
+                                {"startPredictions", startPredictions, METH_VARARGS, nullptr},
                                 {"syncWithHost", syncWithHost, METH_VARARGS, nullptr},
                                 {"startResident", startResident, METH_VARARGS, nullptr},
                                 {"commUniqueId", commUniqueId, METH_NOARGS, nullptr},
                                 {"initComm", initComm, METH_VARARGS, nullptr},
                                 {"setDropoutMasks", setDropoutMasks, METH_VARARGS, nullptr},
                                 {"setSeed", setSeed, METH_VARARGS, nullptr},
+                                {"setGradClip", setGradClip, METH_VARARGS, nullptr},
+                                {"getGradNorm", getGradNorm, METH_NOARGS, nullptr},
                                 {"getActs", getActs, METH_VARARGS, nullptr},
                                 {"setProfile", setProfile, METH_VARARGS, nullptr},
                                 {"getProfile", getProfile, METH_NOARGS, nullptr},
