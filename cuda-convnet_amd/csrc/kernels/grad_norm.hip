@@ -265,8 +265,8 @@ int mc_grad_spans(const mcGradTensor* tensors, int numTensors, mcGradSpan* spans
                 if (spans && n < (unsigned long long)std::max(maxSpans, 0)) spans[n] = sp;
                 ++n;
                 done += sp.count;
+                MC_REQUIRE(fits_a_grid(n * (kSpan / kClipTile), GT), "mc_grad_spans: too many elements");
             }
-            MC_REQUIRE(n <= 0x1fffffffull, "mc_grad_spans: too many elements");
         }
         *numSpans = (int)n;
         MC_REQUIRE(!spans || (unsigned long long)std::max(maxSpans, 0) >= n, "mc_grad_spans: %llu spans, room for %d", n, maxSpans);
@@ -303,7 +303,7 @@ int mc_clip_grads(const mcGradSpan* spansDevice, int numSpans, const float* norm
     MC_REQUIRE(normAndFactor && numSpans >= 0 && (spansDevice || numSpans == 0), "mc_clip_grads: bad arguments");
     MC_REQUIRE(stream_on_current_device(s), "mc_clip_grads: the stream belongs to another device than the current one");
     if (numSpans == 0) return MC_OK;
-    MC_REQUIRE(numSpans <= 0x1fffffff, "mc_clip_grads: too many spans");
+    MC_REQUIRE(fits_a_grid((size_t)numSpans * (kSpan / kClipTile), GT), "mc_clip_grads: too many spans");
     const dim3 grid(numSpans * (kSpan / kClipTile)), block(GT);
     if (spans_stream(numSpans)) hipLaunchKernelGGL(k_clip_grads<true>, grid, block, 0, S(s), spansDevice, normAndFactor);
     else hipLaunchKernelGGL(k_clip_grads<false>, grid, block, 0, S(s), spansDevice, normAndFactor);
@@ -316,6 +316,7 @@ int mc_weights_update_spans_clipped(float* weights, float* inc, const float* gra
     MC_REQUIRE(aligned16(weights) && aligned16(inc) && aligned16(grad), "mc_weights_update_spans_clipped: arenas must be 16-byte aligned");
     MC_REQUIRE(stream_on_current_device(s), "mc_weights_update_spans_clipped: the stream belongs to another device than the current one");
     if (numSpans <= 0) return MC_OK;
+    MC_REQUIRE(fits_a_grid(numSpans, GT), "mc_weights_update_spans_clipped: too many spans");
     if (spans_stream(numSpans)) hipLaunchKernelGGL(k_weights_update_clipped<true>, dim3(numSpans), dim3(GT), 0, S(s), weights, inc, grad, spansDevice, normAndFactor);
     else hipLaunchKernelGGL(k_weights_update_clipped<false>, dim3(numSpans), dim3(GT), 0, S(s), weights, inc, grad, spansDevice, normAndFactor);
     return launch_status("mc_weights_update_spans_clipped");

@@ -1009,34 +1009,40 @@ void launch_log_probs(const Plan& p, const LogProbArgs& a, hipStream_t s) {
 }
 
 template <class T, bool ENT, bool NT>
-void launch_grad_rows(const LogProbGradArgs& g, hipStream_t s) {
+bool launch_grad_rows(const LogProbGradArgs& g, hipStream_t s) {
     constexpr int V = 16 / (int)sizeof(T), U = 4;
     const dim3 block(LT);
     if (g.numOut <= 64 * V * U) {
+        if (!fits_a_grid(ceil_div(g.numCases, LT / 64), LT)) return false;
         const dim3 grid(ceil_div(g.numCases, LT / 64));
         if (g.numOut <= 64 * V) hipLaunchKernelGGL((k_log_probs_grad_rows<T, 64, 1, ENT, NT>), grid, block, 0, s, g, 1);
         else hipLaunchKernelGGL((k_log_probs_grad_rows<T, 64, U, ENT, NT>), grid, block, 0, s, g, 1);
     } else {
         const int parts = ceil_div(g.numOut, LT * V * U);
+        if (!fits_a_grid((size_t)g.numCases * parts, LT)) return false;
         hipLaunchKernelGGL((k_log_probs_grad_rows<T, LT, U, ENT, NT>), dim3((unsigned)((size_t)g.numCases * parts)), block, 0, s, g, parts);
     }
+    return true;
 }
 template <class T, bool ENT, bool NT>
-void launch_grad_cols(const LogProbGradArgs& g, hipStream_t s) {
+bool launch_grad_cols(const LogProbGradArgs& g, hipStream_t s) {
     constexpr int V = 16 / (int)sizeof(T), U = 4;
     const int columns = g.numCases < V ? g.numCases : g.numCases / V + g.numCases % V;
     int logG = 0, rounds = 16;   // (blocks of many rounds, and four of them for each CU)
     while (logG < 4 && (1 << logG) < columns) ++logG;
     const size_t tiles = ceil_div(columns, 1 << logG);
     while (rounds > 1 && tiles * ceil_div(g.numOut, (LT >> logG) * U * rounds) < 4 * (size_t)num_cus()) rounds /= 2;
-    const dim3 block(LT), grid((unsigned)(tiles * ceil_div(g.numOut, (LT >> logG) * U * rounds)));
+    const size_t blocks = tiles * ceil_div(g.numOut, (LT >> logG) * U * rounds);
+    if (!fits_a_grid(blocks, LT)) return false;
+    const dim3 block(LT), grid((unsigned)blocks);
     if (g.numCases < V) hipLaunchKernelGGL((k_log_probs_grad_cols<T, 1, U, ENT, false>), grid, block, 0, s, g, logG, rounds);
     else hipLaunchKernelGGL((k_log_probs_grad_cols<T, V, U, ENT, NT>), grid, block, 0, s, g, logG, rounds);
+    return true;
 }
 template <class T, bool ENT>
-void launch_grad(const LogProbGradArgs& g, bool rows, hipStream_t s) {
-    if (streams((size_t)g.numCases * g.numOut * sizeof(T) * 2)) rows ? launch_grad_rows<T, ENT, true>(g, s) : launch_grad_cols<T, ENT, true>(g, s);
-    else rows ? launch_grad_rows<T, ENT, false>(g, s) : launch_grad_cols<T, ENT, false>(g, s);
+bool launch_grad(const LogProbGradArgs& g, bool rows, hipStream_t s) {
+    if (streams((size_t)g.numCases * g.numOut * sizeof(T) * 2)) return rows ? launch_grad_rows<T, ENT, true>(g, s) : launch_grad_cols<T, ENT, true>(g, s);
+    return rows ? launch_grad_rows<T, ENT, false>(g, s) : launch_grad_cols<T, ENT, false>(g, s);
 }
 
 }  // namespace
@@ -1069,7 +1075,7 @@ int mc_log_probs(const void* logits, int type, long long classStride, long long 
     MC_REQUIRE(labelLogProbs || entropy || maxAndLogSum || numTop, "mc_log_probs: no output asked for");
     MC_REQUIRE(stream_on_current_device(s), "mc_log_probs: the stream belongs to another device than the current one");
     Plan p = plan_log_probs(type, kinds, numCases, numOut, numTop);
-    MC_REQUIRE(p.blocks <= 0x7fffffff, "mc_log_probs: too many cases");
+    MC_REQUIRE(fits_a_grid(p.blocks, LT), "mc_log_probs: too many cases");
     if (p.bytes && (!workspace || workspaceBytes < p.bytes || !aligned16(workspace))) {
         set_error("mc_log_probs: workspace of %zu bytes, 16-byte aligned, needed", p.bytes);
         return MC_EWORKSPACE;
@@ -1114,11 +1120,12 @@ int mc_log_probs_grad(const void* logits, int type, long long classStride, long 
     MC_REQUIRE(stream_on_current_device(s), "mc_log_probs_grad: the stream belongs to another device than the current one");
     const LogProbGradArgs a{logits, (size_t)classStride, (size_t)caseStride, labels, labelType, numCases, numOut, maxAndLogSum, entropy, gradLabel,
                             gradEntropy, gradLogZ, scaleLabel, scaleEntropy, scaleLogZ, target, (size_t)targetClassStride, (size_t)targetCaseStride, add};
+    bool fits = true;
     with_type(type, [&](auto t) {
         typedef decltype(t) T;
-        if (scaleEntropy != 0.f) launch_grad<T, true>(a, kinds & targetKinds & BY_CASE, S(s));
-        else launch_grad<T, false>(a, kinds & targetKinds & BY_CASE, S(s));
+        fits = scaleEntropy != 0.f ? launch_grad<T, true>(a, kinds & targetKinds & BY_CASE, S(s)) : launch_grad<T, false>(a, kinds & targetKinds & BY_CASE, S(s));
     });
+    MC_REQUIRE(fits, "mc_log_probs_grad: too many cases");
     return launch_status("mc_log_probs_grad");
 }
 

@@ -117,6 +117,9 @@ inline bool with_type(int type, F f) {
     return false;
 }
 
+// A launch counts its threads in 32 bits.
+inline bool fits_a_grid(size_t blocks, int threads) { return blocks <= 0xffffffffu / (unsigned)threads; }
+
 // The stream a call names must belong to the current device: every pointer is taken to live there, and grids are sized for it.
 inline bool stream_on_current_device(mcStream_t s) {
     if (!s) return true;

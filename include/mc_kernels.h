@@ -492,7 +492,8 @@ int mc_compute_logreg_softmax_grad(const float* labels, const float* probs, floa
  * (0 for "no class"), entropy 0.  A case with a NaN or +inf logit gets NaN for its log sum, log probabilities and entropy.
  * workspace: mc_log_probs_workspace_bytes(...) bytes (0 = none), 16-byte aligned; calls that may overlap in time, captured ones
  * included, need one each.  Results do not depend on the run: no atomics decide an order.  Outputs must not overlap anything else.
- * The stream must belong to the current device, as must every pointer. */
+ * The stream must belong to the current device, as must every pointer.  Matrices that would take 2^24 workgroups are refused (2^26 cases
+ * side by side, or 2^24 of more classes than a wave holds: 1024 float32 or 2048 16-bit ones). */
 enum { MC_F32 = 0, MC_F16 = 1, MC_BF16 = 2, MC_I32 = 3 };
 #define MC_MAX_TOP 32
 size_t mc_log_probs_workspace_bytes(int type, long long classStride, long long caseStride, int numCases, int numOut, int numTop);

@@ -53,6 +53,18 @@ def test_gradient_refusals(kw, text):
     assert grad(**kw) == -1 and text in last()
 
 
+def test_matrices_that_no_grid_covers_are_refused():
+    assert forward(N=(1 << 26) - 3, V=10, ns=10) == -1 and "too many cases" in last()
+    assert grad(N=(1 << 26) - 3, V=10, ns=10, tns=10, target=1 << 50) == -1 and "too many cases" in last()
+    assert grad(N=1 << 24, V=1 << 15, ns=1 << 15, tns=1 << 15, target=1 << 50) == -1 and "too many cases" in last()
+    assert grad(N=(1 << 31) - 1, V=1 << 20, cs=1 << 31, ns=1, tcs=1 << 31, tns=1, target=1 << 60) == -1 and "too many cases" in last()
+    assert lib().mc_clip_grads(P, 1 << 23, P, None) == -1 and "too many spans" in last()
+    assert lib().mc_weights_update_spans_clipped(P, P, P, P, 1 << 24, P, None) == -1 and "too many spans" in last()
+    import mckernels as m
+    with pytest.raises(m.McError, match="too many elements"):
+        m.grad_spans([(P, 0, 1 << 48, 1.0, 2, 2)])
+
+
 def test_workspace_refusals():
     L = lib()
     assert L.mc_grad_norm(P, 3, 1.0, P, None, 0, None) == -3 and "workspace" in last()
