@@ -172,7 +172,9 @@ __device__ __forceinline__ float top_threshold(const float (&v)[Q], int k, float
     }
     return lo;
 }
-constexpr int kFewClasses = 64;   // so many can all be candidates: ordering them costs less than finding a threshold
+// So many can all be candidates: ordering them costs less than finding a threshold.  (128 class-major cases: 10 classes 5.9 us so and 7.5 with
+// a threshold, 32 classes 9.4 and 7.6.)
+constexpr int kFewClasses = 16;
 
 // The k largest keys of classes [from, to) in one walk over them in order: THREADS classes at a time against the k-th best so far;
 // what beats it joins the list, which is ordered again by counting, for each key, the larger ones.  Any number of ties, any order; used
@@ -206,14 +208,26 @@ __device__ void top_by_scan(const T* x, size_t stride, int from, int to, int k, 
 }
 
 // Orders `count` keys by counting, for each, the larger ones, and gives (rank, key) to `put` for the first k; ranks from count on get
-// key 0.  The keys are distinct, but for zeros where ZEROS says that there may be some.
-template <bool ZEROS, class F>
+// key 0.  The keys are distinct, but for zeros where ZEROS says that there may be some.  A thread takes OWN keys at a time, so that what it
+// reads of the others serves as many.
+template <bool ZEROS, int OWN, class F>
 __device__ __forceinline__ void rank_keys(const unsigned long long* keys, int count, int k, int tid, int threads, F put) {
-    for (int i = tid; i < count; i += threads) {
-        const unsigned long long key = keys[i];
-        int rank = 0;
-        for (int c = 0; c < count; ++c) rank += keys[c] > key || (ZEROS && key == 0 && c < i && keys[c] == 0);
-        if (rank < k) put(rank, key);
+    for (int i = tid; i < count; i += threads * OWN) {
+        unsigned long long key[OWN];
+        int rank[OWN];
+#pragma unroll
+        for (int j = 0; j < OWN; ++j) {
+            key[j] = keys[min(i + j * threads, count - 1)];
+            rank[j] = 0;
+        }
+        for (int c = 0; c < count; ++c) {
+            const unsigned long long other = keys[c];
+#pragma unroll
+            for (int j = 0; j < OWN; ++j) rank[j] += other > key[j] || (ZEROS && key[j] == 0 && c < i + j * threads && other == 0);
+        }
+#pragma unroll
+        for (int j = 0; j < OWN; ++j)
+            if (i + j * threads < count && rank[j] < k) put(rank[j], key[j]);
     }
     for (int r = count + tid; r < k; r += threads) put(r, 0);
 }
@@ -306,12 +320,6 @@ __device__ __forceinline__ float max_in(const Words<T, N>& v, Pass p) {
     for (int i = 1; i < v.COUNT; ++i) asm("v_pk_max_f16 %0, %1, %2" : "=v"(m.w[0]) : "v"(m.w[0]), "v"(v.w[i]));
     return fmaxf(m.at(0, p), m.at(1, p));
 }
-// The larger of two pairs of 16-bit integers, half by half.
-__device__ __forceinline__ unsigned max_pairs(unsigned a, unsigned b) {
-    unsigned r;
-    asm("v_pk_max_i16 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
-    return r;
-}
 // Element k as fma(x, scale, -c); a half goes into the fma as it is (volatile: see Pass).
 template <class T, int N>
 __device__ __forceinline__ float shifted(const Words<T, N>& v, int k, Shift h, Pass p) {
@@ -372,37 +380,16 @@ __global__ void __launch_bounds__(LT) __attribute__((amdgpu_waves_per_eu(4))) k_
     if (a.labelLogProbs) label = label_of(a.labels, a.labelType, n, a.numOut);
     const float labelLogit = label >= lo && label < lo + len ? (float)x[label - lo] : -INFINITY;
 
-    // The packs' maxima.  bf16: as pairs of 16-bit integers first, in whose order non-negative numbers are, and below them the negative ones,
-    // backwards; where the group's largest is not negative (nor infinite, nor NaN), it is right, and a pack's is right if it is not negative
-    // and too low otherwise.  Half the instructions of taking the pairs apart.
-    constexpr bool PAIRS = __is_same(T, __bf16);
-    unsigned pw[U];
-    const auto pm = [&](int u) { return __uint_as_float(pw[u]); };
-    const auto find_maxima = [&] {
+    // The packs' maxima.  (bf16 as pairs of 16-bit integers takes half the instructions, but only where the largest is not negative, and was no
+    // faster: 2048 x 131072 97 ... 103 us, this 95 ... 103.)
+    float pm[U];
+    {
         const Pass pass;
 #pragma unroll
-        for (int u = 0; u < U; ++u) pw[u] = __float_as_uint(max_in(v[u], pass));
-        return max_of<U>(pm);
-    };
-    float mine = 0.f, m = 0.f;
-    bool pairs = false;
-    if (PAIRS) {
-        unsigned all = 0;
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            pw[u] = max_pairs(max_pairs(v[u].w[0], v[u].w[1]), max_pairs(v[u].w[2], v[u].w[3]));
-            all = u ? max_pairs(all, pw[u]) : pw[u];
-        }
-        const int i = max((int)(short)all, (int)all >> 16);
-        mine = i > 0x7f7f ? INFINITY : __int_as_float(i << 16);
-        m = G::max(mine, shRed[group]);
-        pairs = m >= 0.f && m < kHuge;
-        if (!pairs) G::sync();
+        for (int u = 0; u < U; ++u) pm[u] = max_in(v[u], pass);
     }
-    if (!pairs) {
-        mine = find_maxima();
-        m = G::max(mine, shRed[group]);
-    }
+    const float mine = max_of<U>([&](int u) { return pm[u]; });
+    const float m = G::max(mine, shRed[group]);
     if (TOP) {
         shMax[threadIdx.x] = mine;
         if (tid == 0) shCount[group] = shPacks[group] = 0;
@@ -433,15 +420,9 @@ __global__ void __launch_bounds__(LT) __attribute__((amdgpu_waves_per_eu(4))) k_
 #pragma unroll
     for (int i = 0; i < THREADS / 64; ++i) q[i] = shMax[group * THREADS + i * 64 + (threadIdx.x & 63)];
     const float threshold = len <= kFewClasses ? -INFINITY : top_threshold(q, a.numTop, m, 64);
-    if (pairs && !(threshold > 0.f)) {
-        find_maxima();
-        pairs = false;
-    }
-    // (reaching a positive threshold is, for the pairs, exceeding the bf16 below it)
-    const unsigned under = ((__float_as_uint(threshold) + 0xffffu) >> 16) - 1, below = under << 16 | (under & 0xffffu);
 #pragma unroll
     for (int u = 0; u < U; ++u)
-        if (pairs ? max_pairs(pw[u], below) != below : pm(u) >= threshold && pm(u) > -INFINITY) {
+        if (pm[u] >= threshold && pm[u] > -INFINITY) {
             const int to = atomicAdd(&shPacks[group], 1);
             if (to < PACKS) {
 #pragma unroll
@@ -467,7 +448,7 @@ __global__ void __launch_bounds__(LT) __attribute__((amdgpu_waves_per_eu(4))) k_
         if (p.parts == 1) write_top(a, n, rank, key, c);
         else p.keys[(size_t)item * a.numTop + rank] = key;
     };
-    if (packs <= PACKS && count <= kCand) rank_keys<false>(shCand[group], count, a.numTop, tid, THREADS, put);
+    if (packs <= PACKS && count <= kCand) rank_keys<false, 1>(shCand[group], count, a.numTop, tid, THREADS, put);
     else {   // ties, or orders that put many of the largest into few packs' reach
         G::sync();
         top_by_scan<THREADS>(x - lo, 1, lo, lo + len, a.numTop, shCand[group] + kCand, shCand[group]);
@@ -583,7 +564,7 @@ __global__ void __launch_bounds__(LT) k_log_probs_cols(LogProbArgs a, Parts p, i
 
     const int lanes = min(64, LT / cases), owner = threadIdx.x / lanes, sub = threadIdx.x % lanes, stretches = WINDOWS * R, cap = col_cand(a.numTop);
     const int len = hi - lo;
-    const bool few = len <= kFewClasses / 2;   // then each class has a place in its cases' lists
+    const bool few = len <= kFewClasses;   // then each class has a place in its cases' lists
     const Pass third;
     if (few) {
 #pragma unroll
@@ -628,7 +609,11 @@ __global__ void __launch_bounds__(LT) k_log_probs_cols(LogProbArgs a, Parts p, i
         else p.keys[((size_t)n * p.parts + part) * a.numTop + rank] = key;
     };
     const int count = owner < cases ? few ? len : shCount[owner] : 0;
-    if (owner < cases && count <= cap) rank_keys<true>(shDyn + owner * cap, count, a.numTop, sub, lanes, [&](int rank, unsigned long long key) { put(owner, rank, key); });
+    if (owner < cases && count <= cap) {
+        const auto own = [&](int rank, unsigned long long key) { put(owner, rank, key); };
+        if (few) rank_keys<true, 2>(shDyn + owner * cap, count, a.numTop, sub, lanes, own);
+        else rank_keys<false, U == 16 ? 4 : 1>(shDyn + owner * cap, count, a.numTop, sub, lanes, own);   // (32000 x 2048 f32: 148 us with 1 at a time, 115 with 4)
+    }
     if (!__syncthreads_or(count > cap)) return;
     for (int cc = 0; cc < cases; ++cc) {   // lists that overflowed: the lists' memory is free by now
         if (shCount[cc] <= cap) continue;
@@ -640,21 +625,25 @@ __global__ void __launch_bounds__(LT) k_log_probs_cols(LogProbArgs a, Parts p, i
 }
 
 // ---------------------------------------------------------------- joining the parts of a case
-constexpr int kJoinCand = 1024;
+// A wave joins up to 16 parts, whose keys it holds at once: the threshold is found from all of them.  Beyond, a workgroup does: a first
+// threshold from the parts' best keys (or their last ones, where there are few parts), a better one from what reaches that.  (Ordering what
+// only the first lets through took most of the time: 16 parts of 20 keys each 19.7 us.)
+constexpr int kJoinWave = 16, kJoinCand = 1024, kJoinFew = 128;
 template <int THREADS>
 __global__ void __launch_bounds__(LT) k_log_probs_join(LogProbArgs a, Parts p) {
     typedef Group<THREADS> G;
-    constexpr int GROUPS = LT / THREADS, CAND = THREADS == 64 ? kJoinCand / 4 : kJoinCand;
+    constexpr int GROUPS = LT / THREADS, CAND = THREADS == 64 ? kJoinFew : kJoinCand;
     __shared__ float shRed[GROUPS][4 * G::WAVES];
     __shared__ unsigned long long shCand[GROUPS][CAND];
-    __shared__ int shCount[GROUPS];
+    __shared__ unsigned long long shBest[THREADS == LT ? kJoinFew : 1];
+    __shared__ int shCount[GROUPS], shBestCount;
     const int group = G::index(), tid = G::tid();
     const size_t row = (size_t)blockIdx.x * GROUPS + group;
     if (row >= (size_t)a.numCases) return;
     const int n = (int)row;
     // All that is read is under way before anything is waited for: statistics, label, the parts' best keys, and as many of all keys as the
     // threads hold at EARLY each.
-    constexpr int EARLY = 6;
+    constexpr int EARLY = THREADS == 64 ? kJoinWave * MC_MAX_TOP / 64 : 6;
     const Part* stats = p.stats + row * p.parts;
     const unsigned long long* keys = p.keys + row * p.parts * a.numTop;
     const int total = p.parts * a.numTop;
@@ -662,17 +651,17 @@ __global__ void __launch_bounds__(LT) k_log_probs_join(LogProbArgs a, Parts p) {
     if (tid < p.parts) part = stats[tid];
     int label = -1;
     if (a.labelLogProbs) label = label_of(a.labels, a.labelType, n, a.numOut);
-    const unsigned long long tail = a.numTop && tid < p.parts ? keys[(size_t)(tid + 1) * a.numTop - 1] : 0;
+    const unsigned long long tail = THREADS == LT && a.numTop && tid < p.parts ? keys[(size_t)(tid + 1) * a.numTop - 1] : 0;
     unsigned long long early[EARLY];
 #pragma unroll
     for (int i = 0; i < EARLY; ++i) early[i] = tid + i * THREADS < total ? keys[tid + i * THREADS] : 0;
-    const bool thresholds = p.parts > a.numTop && total > kFewClasses;
+    const bool thresholds = THREADS == LT && p.parts > a.numTop;
     constexpr int Q = 8;
     unsigned long long head[Q];
     const int heads = min(p.parts, 64 * Q);   // (beyond: the first ones' threshold holds too)
 #pragma unroll
     for (int i = 0; i < Q; ++i) head[i] = thresholds && (int)(threadIdx.x & 63) + 64 * i < heads ? keys[(size_t)((threadIdx.x & 63) + 64 * i) * a.numTop] : 0;
-    if (tid == 0) shCount[group] = 0;
+    if (tid == 0) shCount[group] = shBestCount = 0;
     float m = part.m, labelLogit = part.label;
     for (int i = tid + THREADS; i < p.parts; i += THREADS) {
         m = fmaxf(m, stats[i].m);
@@ -694,12 +683,17 @@ __global__ void __launch_bounds__(LT) k_log_probs_join(LogProbArgs a, Parts p) {
 
     // candidates: keys that reach a value that numTop parts' best keys reach
     float threshold = -INFINITY;
-    if (thresholds) {
+    if (THREADS == 64) {
+        float q[EARLY];
+#pragma unroll
+        for (int i = 0; i < EARLY; ++i) q[i] = early[i] ? key_logit(early[i]) : -INFINITY;
+        threshold = total > kFewClasses ? top_threshold(q, a.numTop, m, 64) : -INFINITY;
+    } else if (thresholds) {
         float q[Q];
 #pragma unroll
         for (int i = 0; i < Q; ++i) q[i] = head[i] ? key_logit(head[i]) : -INFINITY;
         threshold = top_threshold(q, a.numTop, m, 64);
-    } else if (total > kFewClasses / 2) {   // few parts: the last key of any part's list has numTop keys from it up
+    } else {   // few parts: the last key of any part's list has numTop keys from it up
         float last = tid < p.parts && tail ? key_logit(tail) : -INFINITY;
         threshold = over_lanes(last, 1, Larger());   // (in the first wave; parts <= numTop are all there, and the others' -inf is a threshold too)
     }
@@ -712,11 +706,32 @@ __global__ void __launch_bounds__(LT) k_log_probs_join(LogProbArgs a, Parts p) {
     G::sync();
 #pragma unroll
     for (int i = 0; i < EARLY; ++i) take(early[i]);
-    for (int i = tid + EARLY * THREADS; i < total; i += THREADS) take(keys[i]);
+    if (THREADS == LT)
+        for (int i = tid + EARLY * THREADS; i < total; i += THREADS) take(keys[i]);
     G::sync();
-    const int count = shCount[group];
+    int count = shCount[group];
     if (count <= CAND) {
-        rank_keys<false>(shCand[group], count, a.numTop, tid, THREADS, [&](int rank, unsigned long long key) { write_top(a, n, rank, key, c); });
+        const unsigned long long* list = shCand[group];
+        if (THREADS == LT && count > kJoinFew) {
+            float q[CAND / 64];
+#pragma unroll
+            for (int i = 0; i < CAND / 64; ++i) {
+                const int at = i * 64 + (threadIdx.x & 63);
+                q[i] = at < count ? key_logit(list[at]) : -INFINITY;
+            }
+            const float better = top_threshold(q, a.numTop, m, 64);
+            for (int i = tid; i < count; i += THREADS)
+                if (key_logit(list[i]) >= better) {
+                    const int to = atomicAdd(&shBestCount, 1);
+                    if (to < kJoinFew) shBest[to] = list[i];
+                }
+            G::sync();
+            if (shBestCount <= kJoinFew) {
+                list = shBest;
+                count = shBestCount;
+            }
+        }
+        rank_keys<false, 1>(list, count, a.numTop, tid, THREADS, [&](int rank, unsigned long long key) { write_top(a, n, rank, key, c); });
         return;
     }
     // more ties than the list holds: the best, then the best below it, and so on
@@ -856,14 +871,14 @@ __global__ void __launch_bounds__(LT) k_log_probs_grad_rows(LogProbGradArgs g, i
     }
 }
 
-// A lane takes P neighbouring cases of `rounds` times U classes; the cases that fill no pack are taken one a lane (P = 1) by the lanes
+// A lane takes P neighbouring cases of U classes; the cases that fill no pack are taken one a lane (P = 1) by the lanes
 // behind the packs'.  What a case needs is loaded once for all of a lane's classes.
 template <class T, int P, int U, bool ENT, bool NT>
-__global__ void __launch_bounds__(LT) k_log_probs_grad_cols(LogProbGradArgs g, int logG, int rounds) {
+__global__ void __launch_bounds__(LT) k_log_probs_grad_cols(LogProbGradArgs g, int logG) {
     const int G = 1 << logG, R = LT >> logG, packs = g.numCases / P, columns = packs + g.numCases % P;
     const int tiles = (columns + G - 1) >> logG;
     const int column = ((int)(blockIdx.x % tiles) << logG) + (threadIdx.x & (G - 1));
-    const int from = (int)(blockIdx.x / tiles) * (R * U * rounds) + (threadIdx.x >> logG), to = min(from + R * U * rounds, g.numOut);
+    const int j0 = (int)(blockIdx.x / tiles) * (R * U) + (threadIdx.x >> logG);
     if (column >= columns) return;
     const T* logits = static_cast<const T*>(g.logits);
     T* target = static_cast<T*>(g.target);
@@ -871,34 +886,32 @@ __global__ void __launch_bounds__(LT) k_log_probs_grad_cols(LogProbGradArgs g, i
         constexpr int N = decltype(width)::value;
         const T* x = logits + (size_t)n0 * (P == 1 ? g.caseStride : 1);
         T* out = target + (size_t)n0 * (P == 1 ? g.targetCaseStride : 1);
+        Words<T, N> v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u].template load<NT>(x + (size_t)min(j0 + u * R, g.numOut - 1) * g.classStride);
         CaseGrad c[N];
         case_grads<ENT>(g, n0, c);
-        for (int j0 = from; j0 < to; j0 += R * U) {
-            Words<T, N> v[U];
+        bool here = false;   // is a label of these cases among these classes, or between them?
 #pragma unroll
-            for (int u = 0; u < U; ++u) v[u].template load<NT>(x + (size_t)min(j0 + u * R, g.numOut - 1) * g.classStride);
-            bool here = false;   // is a label of these cases among these classes, or between them?
+        for (int k = 0; k < N; ++k) here |= (unsigned)(c[k].y - j0) < (unsigned)(R * U);
+        const Pass pass;
 #pragma unroll
-            for (int k = 0; k < N; ++k) here |= (unsigned)(c[k].y - j0) < (unsigned)(R * U);
-            const Pass pass;
+        for (int u = 0; u < U; ++u) {
+            const int j = j0 + u * R;
+            Words<T, N> t;
+            if (g.add) t.template load<NT>(out + (size_t)min(j, g.numOut - 1) * g.targetClassStride);
+            Pack<T, N> d;
+            float e[N];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int j = j0 + u * R;
-                Words<T, N> t;
-                if (g.add) t.template load<NT>(out + (size_t)min(j, g.numOut - 1) * g.targetClassStride);
-                Pack<T, N> d;
-                float e[N];
+            for (int k = 0; k < N; ++k) e[k] = grad_of<ENT>(v[u].at(k, pass), c[k]);
+            if (here) {
 #pragma unroll
-                for (int k = 0; k < N; ++k) e[k] = grad_of<ENT>(v[u].at(k, pass), c[k]);
-                if (here) {
-#pragma unroll
-                    for (int k = 0; k < N; ++k)
-                        if (j == c[k].y) e[k] += c[k].a;
-                }
-#pragma unroll
-                for (int k = 0; k < N; ++k) d.v[k] = (T)(g.add ? e[k] + t.at(k, pass) : e[k]);
-                if (j < to) store_pack<NT, T, N>(out + (size_t)j * g.targetClassStride, d);
+                for (int k = 0; k < N; ++k)
+                    if (j == c[k].y) e[k] += c[k].a;
             }
+#pragma unroll
+            for (int k = 0; k < N; ++k) d.v[k] = (T)(g.add ? e[k] + t.at(k, pass) : e[k]);
+            if (j < g.numOut) store_pack<NT, T, N>(out + (size_t)j * g.targetClassStride, d);
         }
     };
     if (P > 1 && column >= packs) take(std::integral_constant<int, 1>(), packs * P + (column - packs));
@@ -964,8 +977,8 @@ Plan plan_log_probs(int type, int kinds, int numCases, int numOut, int numTop) {
         for (p.U = small ? 1 : 16; small && LT * p.U < numOut; p.U *= 4) {}
         while (p.logG < most && (p.P << p.logG) < numCases && (!small || (LT >> (p.logG + 1)) * p.U >= numOut)) ++p.logG;
         const int R = LT >> p.logG, tiles = ceil_div(numCases, p.P << p.logG);
-        if (!small)   // (up to 128 parts, or joining them takes longer than what it gains)
-            for (; p.U > 1 && (numOut <= R * (p.U / 4) || ((size_t)tiles * ceil_div(numOut, R * p.U) < 2 * (size_t)cus && ceil_div(numOut, R * (p.U / 4)) <= 128)); p.U /= 4) {}
+        if (!small)   // (up to 256 parts, or joining them takes longer than what it gains)
+            for (; p.U > 1 && (numOut <= R * (p.U / 4) || ((size_t)tiles * ceil_div(numOut, R * p.U) < 2 * (size_t)cus && ceil_div(numOut, R * (p.U / 4)) <= 256)); p.U /= 4) {}
         p.parts.span = R * p.U;
         p.parts.parts = ceil_div(numOut, p.parts.span);
         p.blocks = (size_t)tiles * p.parts.parts;
@@ -1003,8 +1016,7 @@ void launch_log_probs(const Plan& p, const LogProbArgs& a, hipStream_t s) {
     if (streams((size_t)a.numCases * a.numOut * sizeof(T))) launch_parts<T, ENT, TOP, true>(p, a, s);
     else launch_parts<T, ENT, TOP, false>(p, a, s);
     if (p.parts.parts == 1) return;
-    // a wave joins up to 16 parts; cases of many parts take a workgroup each
-    if (p.parts.parts <= 16) hipLaunchKernelGGL((k_log_probs_join<64>), dim3(ceil_div(a.numCases, LT / 64)), dim3(LT), 0, s, a, p.parts);
+    if (p.parts.parts <= kJoinWave) hipLaunchKernelGGL((k_log_probs_join<64>), dim3(ceil_div(a.numCases, LT / 64)), dim3(LT), 0, s, a, p.parts);
     else hipLaunchKernelGGL((k_log_probs_join<LT>), dim3(a.numCases), dim3(LT), 0, s, a, p.parts);
 }
 
@@ -1026,17 +1038,16 @@ bool launch_grad_rows(const LogProbGradArgs& g, hipStream_t s) {
 }
 template <class T, bool ENT, bool NT>
 bool launch_grad_cols(const LogProbGradArgs& g, hipStream_t s) {
-    constexpr int V = 16 / (int)sizeof(T), U = 4;
+    constexpr int V = 16 / (int)sizeof(T), U = 2;
     const int columns = g.numCases < V ? g.numCases : g.numCases / V + g.numCases % V;
-    int logG = 0, rounds = 16;   // (blocks of many rounds, and four of them for each CU)
-    while (logG < 4 && (1 << logG) < columns) ++logG;
+    int logG = 0;
+    while (logG < 6 && (1 << logG) < columns) ++logG;
     const size_t tiles = ceil_div(columns, 1 << logG);
-    while (rounds > 1 && tiles * ceil_div(g.numOut, (LT >> logG) * U * rounds) < 4 * (size_t)num_cus()) rounds /= 2;
-    const size_t blocks = tiles * ceil_div(g.numOut, (LT >> logG) * U * rounds);
+    const size_t blocks = tiles * ceil_div(g.numOut, (LT >> logG) * U);
     if (!fits_a_grid(blocks, LT)) return false;
     const dim3 block(LT), grid((unsigned)blocks);
-    if (g.numCases < V) hipLaunchKernelGGL((k_log_probs_grad_cols<T, 1, U, ENT, false>), grid, block, 0, s, g, logG, rounds);
-    else hipLaunchKernelGGL((k_log_probs_grad_cols<T, V, U, ENT, NT>), grid, block, 0, s, g, logG, rounds);
+    if (g.numCases < V) hipLaunchKernelGGL((k_log_probs_grad_cols<T, 1, U, ENT, false>), grid, block, 0, s, g, logG);
+    else hipLaunchKernelGGL((k_log_probs_grad_cols<T, V, U, ENT, NT>), grid, block, 0, s, g, logG);
     return true;
 }
 template <class T, bool ENT>
