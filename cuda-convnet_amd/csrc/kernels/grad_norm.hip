@@ -83,6 +83,8 @@ __device__ __forceinline__ double span_square(const mcGradSpan& sp, bool nt) {
     return nt ? span_square<T, true>(g, sp.count) : span_square<T, false>(g, sp.count);
 }
 
+// One read of every gradient, bound by HBM: 2^28 bf16 in 300 tensors 87 us (6.2 TB/s), 2^27 f32 in 120 82 (6.6).  (16-bit numbers: the vector
+// units are nearly as busy.)  As many workgroups as the second pass can add up in one go, each over spans a grid apart.
 __global__ void __launch_bounds__(GT) k_grad_square(const mcGradSpan* __restrict__ spans, int numSpans, double* __restrict__ partials, bool nt) {
     __shared__ double sh[GT / 64];
     double acc = 0.0;
@@ -115,7 +117,7 @@ __global__ void __launch_bounds__(GT) k_grad_factor(const double* __restrict__ p
 }
 
 // kClipPacks packs of 4 elements a thread: a workgroup takes a part of a span.  (Streams of small tiles in the order of memory copy faster
-// than workgroups that walk through stretches of their own.)
+// than workgroups that walk through stretches of their own.)  2^28 bf16 into f32 (1.6 GB) 267 us, 6.0 TB/s.
 constexpr int kClipPacks = 2, kClipTile = GT * 4 * kClipPacks;
 template <bool NT, class T, class O>
 __device__ __forceinline__ void tile_scale(const T* g, O* out, unsigned at, unsigned n, float f) {
@@ -168,7 +170,7 @@ __device__ __forceinline__ void step(float& w, float& i, float g, float f, float
     if (wceps != 0.f) i = fmaf(wceps, w, i);
     w += i;
 }
-// A workgroup takes a span, with up to 12 loads in flight a thread.
+// A workgroup takes a span, with up to 12 loads in flight a thread.  Three reads and two writes of HBM: 2^27 weights (2.7 GB) 469 us, 5.7 TB/s.
 template <bool NT>
 __global__ void __launch_bounds__(GT) __attribute__((amdgpu_waves_per_eu(8)))
 k_weights_update_clipped(float* w, float* inc, const float* __restrict__ grad, const mcUpdateSpan* __restrict__ spans, const float* __restrict__ normAndFactor) {

@@ -332,7 +332,9 @@ __device__ __forceinline__ float shifted(const Words<T, N>& v, int k, Shift h, P
 
 // ---------------------------------------------------------------- a case's classes side by side
 // A workgroup (or wave) takes up to THREADS * U packs of 16 bytes of one case into registers in one burst of loads, and does all the
-// rest there: the largest logit, the sums against it, the candidates for the top.
+// rest there: the largest logit, the sums against it, the candidates for the top.  One pass over memory, and no rescaling of running
+// sums.  Long cases are bound by HBM with the vector units close behind (7 instructions an element, 80 ... 90 % busy): 2048 x 131072 bf16
+// (537 MB) with entropy and 20 alternatives 90 ... 100 us and 8 for joining, 5.0 ... 5.5 TB/s; reading alone takes 78.
 constexpr int kPacks = 128;
 template <class T, int THREADS, int U, bool ENT, bool TOP, bool NT>
 __global__ void __launch_bounds__(LT) __attribute__((amdgpu_waves_per_eu(4))) k_log_probs_rows(LogProbArgs a, Parts p) {
@@ -458,7 +460,10 @@ __global__ void __launch_bounds__(LT) __attribute__((amdgpu_waves_per_eu(4))) k_
 
 // ---------------------------------------------------------------- a class's cases side by side
 // A workgroup takes 256 / G classes of G * P cases at a time, U times, into registers: lane (r, g) holds P neighbouring cases of class
-// r of each.  P states a lane are reduced over the lanes that share them, then over the waves.
+// r of each.  P states a lane are reduced over the lanes that share them, then over the waves.  Without alternatives HBM bounds it (32000 x
+// 2048 bf16, 131 MB, 34 us and 5 for joining); with them every workgroup looks for the best of each of its cases among few classes, which
+// takes the vector units longer than the loads: the same with 20 alternatives 94 and 12 (16 more for keeping the stretches' maxima, 7
+// for thresholds, 31 for collecting what reaches them, 6 for ordering it).
 // LDS of the top alternatives: the candidate lists (or what top_by_scan needs), the stretches' maxima, the counts, the thresholds.  A list
 // holds what a threshold lets through with room to spare: of s stretches, k of whose maxima reach it, about s ln(s / (s - k)) classes do.
 __host__ __device__ constexpr int col_cand(int top) { return 2 * top + 32; }
@@ -625,7 +630,7 @@ __global__ void __launch_bounds__(LT) k_log_probs_cols(LogProbArgs a, Parts p, i
 }
 
 // ---------------------------------------------------------------- joining the parts of a case
-// A wave joins up to 16 parts, whose keys it holds at once: the threshold is found from all of them.  Beyond, a workgroup does: a first
+// A wave joins up to 16 parts (2048 cases of 4: 8 us, a workgroup each 9), whose keys it holds at once: the threshold is found from all of them.  Beyond, a workgroup does: a first
 // threshold from the parts' best keys (or their last ones, where there are few parts), a better one from what reaches that.  (Ordering what
 // only the first lets through took most of the time: 16 parts of 20 keys each 19.7 us.)
 constexpr int kJoinWave = 16, kJoinCand = 1024, kJoinFew = 128;
@@ -768,7 +773,8 @@ struct LogProbGradArgs {
     int add;
 };
 
-// d_j = p_j (A - h (ln p_j + H)) + [j = y] a
+// d_j = p_j (A - h (ln p_j + H)) + [j = y] a.  Each logit is read and each gradient written once: bound by HBM.  2048 x 131072 bf16
+// (1.07 GB) 176 us, 6.1 TB/s; 511 x 50021 f32 (204 MB) 38.
 struct CaseGrad { float m, logSum, A, h, H, a; int y; };
 // A case's weights, of N neighbouring cases.
 template <int N>
@@ -834,6 +840,7 @@ __device__ __forceinline__ Pack<T, N> grad_pack(const Words<T, N>& v, const Word
     return d;
 }
 
+// U = 4 packs a thread: 2048 x 131072 bf16 178 us; with 2 187, with 8 183.
 template <class T, int THREADS, int U, bool ENT, bool NT>
 __global__ void __launch_bounds__(LT) k_log_probs_grad_rows(LogProbGradArgs g, int parts) {
     typedef Group<THREADS> G;
@@ -872,7 +879,9 @@ __global__ void __launch_bounds__(LT) k_log_probs_grad_rows(LogProbGradArgs g, i
 }
 
 // A lane takes P neighbouring cases of U classes; the cases that fill no pack are taken one a lane (P = 1) by the lanes
-// behind the packs'.  What a case needs is loaded once for all of a lane's classes.
+// behind the packs'.  What a case needs is loaded once for all of a lane's classes.  Up to 64 lanes side by side, so that a wave's accesses
+// make whole lines: 50021 x 511 f32 51 us, 62 with 32 lanes, 78 with 16.  U = 2: 48, and 1000 x 128 3.3 us against 3.7 with 4 (32000 x 2048
+// bf16: 49 against 47).
 template <class T, int P, int U, bool ENT, bool NT>
 __global__ void __launch_bounds__(LT) k_log_probs_grad_cols(LogProbGradArgs g, int logG) {
     const int G = 1 << logG, R = LT >> logG, packs = g.numCases / P, columns = packs + g.numCases % P;
@@ -938,8 +947,10 @@ int check_labels(const char* what, const void* labels, int labelType, int numOut
 }
 
 // ---------------------------------------------------------------- how a call is cut up
-// Logits with a case's classes side by side: up to 64 * 4 packs of 16 bytes a wave takes a case, beyond a workgroup, and a case is split
-// where it is longer than 256 * 16 packs or where there are too few cases to fill the device.  Class-major logits: see below.
+// Logits with a case's classes side by side: up to 64 * 4 packs of 16 bytes a wave takes a case, beyond a workgroup (8192 x 1000 f32:
+// 12.4 us, a workgroup each 21.5), and a case is split where it is longer than 256 * 16 packs or where there are too few cases to fill
+// the device: 16 packs a thread where that still makes 4 workgroups a CU, else 4 where that makes one, else 1 (257 x 50021 f16 14.3 us
+// in parts of 4 packs a thread, 17.6 in parts of 16; 128 x 131072 bf16 12.6 and 13.7).  Class-major logits: see below.
 struct Plan {
     bool rows;
     int threads;   // rows: of a group
@@ -971,13 +982,13 @@ Plan plan_log_probs(int type, int kinds, int numCases, int numOut, int numTop) {
         p.P = V;
         if (numCases < p.P) p.P = 1;
         // A small matrix: every case in one part, if a workgroup of R classes by 1 ... 16 can hold it.  (Its lines are then read in short
-        // pieces, which the L2 makes up for; joining costs a launch.)
+        // pieces, which the L2 makes up for; joining costs a launch: 1000 x 128 f32 9.5 us, split 15.2; 4000 x 128 16.9 and 16.1.)
         const bool small = (size_t)numCases * numOut * elem_size(type) <= (4u << 20) && numOut <= LT * 16;
-        const int most = numTop && p.P == 8 ? 2 : 3;   // (32 cases' candidates to a workgroup, of 64 classes at a time)
+        const int most = numTop && p.P == 8 ? 2 : 3;   // (32 cases' candidates to a workgroup, of 64 classes at a time: 32000 x 2048 bf16 109 us, with 64 cases 200)
         for (p.U = small ? 1 : 16; small && LT * p.U < numOut; p.U *= 4) {}
         while (p.logG < most && (p.P << p.logG) < numCases && (!small || (LT >> (p.logG + 1)) * p.U >= numOut)) ++p.logG;
         const int R = LT >> p.logG, tiles = ceil_div(numCases, p.P << p.logG);
-        if (!small)   // (up to 256 parts, or joining them takes longer than what it gains)
+        if (!small)   // (up to 256 parts, or joining them takes longer than what it gains: 131072 x 4 bf16 16.4 us in 128 parts, 23.8 in 512)
             for (; p.U > 1 && (numOut <= R * (p.U / 4) || ((size_t)tiles * ceil_div(numOut, R * p.U) < 2 * (size_t)cus && ceil_div(numOut, R * (p.U / 4)) <= 256)); p.U /= 4) {}
         p.parts.span = R * p.U;
         p.parts.parts = ceil_div(numOut, p.parts.span);
