@@ -185,6 +185,22 @@ def test_ties_and_orders(N, V, layout):
                 check(x, y, top, forward(x, y, top))
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("N,V", [(2, 3000), (2, 16384), (2, 24000), (2, 33000), (2, 40000), (2, 300000), (300, 33000)])
+def test_joined_parts(N, V, kind):
+    """Cases split into few parts and many: more parts than alternatives and fewer, ties beyond the joining kernels' lists, one part that holds
+    all of the best, parts that hold nothing."""
+    rng = np.random.default_rng(V)
+    rows = [np.zeros(V), np.arange(V) // 64 * 1.0, np.where(np.arange(V) % 5 == 0, 1.0, -2.0), np.where(np.arange(V) < 40, 9.0 + np.arange(V) / 64.0, 0.0),
+            np.where(np.arange(V) >= V - 3, 2.0, -INF), np.where(np.arange(V) % 1000 == 7, np.arange(V) % 7.0, -INF), rng.standard_normal(V), np.floor(3 * rng.standard_normal(V))]
+    for i in range(0, len(rows), min(N, len(rows))):
+        v = np.resize(np.stack(rows[i:i + N]), (N, V))
+        for top in (1, 5, 20, 32) if N == 2 else (20,):
+            x = Matrix(v, kind, "case")
+            y = np.arange(N) % V
+            check(x, y, top, forward(x, y, top))
+
+
 @pytest.mark.parametrize("layout", ["class", "case"])
 def test_offsets_beyond_32_bits(layout):
     """Lines further apart than 2^32 bytes (and elements)."""
