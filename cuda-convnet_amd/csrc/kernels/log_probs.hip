@@ -220,6 +220,7 @@ __device__ __forceinline__ void rank_keys(const unsigned long long* keys, int co
             key[j] = keys[min(i + j * threads, count - 1)];
             rank[j] = 0;
         }
+#pragma unroll 8   // (several reads of the LDS under way: 1 x 131072 bf16 10.3 -> 9.6 us)
         for (int c = 0; c < count; ++c) {
             const unsigned long long other = keys[c];
 #pragma unroll
