@@ -39,6 +39,7 @@ def main():
     ap.add_argument("--single-rank-comm", type=int, default=0)
     ap.add_argument("--predict", default="", help="layer name: its features, and predictions from it with --top alternatives")
     ap.add_argument("--top", type=int, default=0)
+    ap.add_argument("--between", type=int, default=0, help="predictions of that many cases after each batch of --clips")
     ap.add_argument("--out", required=True)
     a = ap.parse_args()
     import libkernel
@@ -89,6 +90,7 @@ def main():
         if b == a.poison:
             d[0][:, 0] = np.nan
         libkernel.startBatch(d, 0)
+        refused(RuntimeError, libkernel.setGradClip, 7.0)       # a batch is under way
         res["case:%d" % b] = libkernel.finishBatch()[1]
         if c in ("keep", "0"):
             refused(RuntimeError, libkernel.getGradNorm)
@@ -97,6 +99,12 @@ def main():
             norms.append(libkernel.getGradNorm())
         libkernel.syncWithHost()
         weights(layers, res, str(b))
+        if a.between:
+            out = np.full((a.between, 2 + 2 * 3), np.nan, np.float32)
+            soft = [i for i, l in enumerate(layers) if l["type"] == "softmax"][0]
+            libkernel.startPredictions([np.ascontiguousarray(x[:, :a.between]) for x in data] + [out], soft, 3)
+            res["cost:%d" % b] = libkernel.finishBatch()[0]["logprob"]
+            res["out:%d" % b] = out
     prof = libkernel.getProfile()
     np.savez(a.out, norms=np.array(norms), replays=prof["net/step_graph:replays"][0], forked=prof["net/step_fork:steps"][0], **res)
 

@@ -139,6 +139,23 @@ def test_predictions(net, layer, top):
     assert (r["out"][:, 2 + k:2 + top] == -1).all() and (r["out"][:, 2 + top + k:] == -np.inf).all()
 
 
+@pytest.mark.parametrize("env", [{"MC_NO_STEP_GRAPH": "1"}, {"MC_STEP_GRAPH": "1"}])
+def test_predictions_between_training_batches(env):
+    """Training goes on to the same bits whether or not the net predicts in between (another number of cases, so that matrices change
+    shape under captured steps), and what it predicts is what the cost layer of the same pass saw: the log probabilities add up to its
+    cost. A case's bound: 156 U for the log probability (test_predictions' for 10 classes, |ln p| < 5); for the cost a probability off by 100 U
+    (a float32 exp of |x - m| < 16 as x and m are rounded, a sum of 10, a division) and a logarithm off by 2 U of 5: below 280 U. Sums are in double."""
+    kw = dict(net="80sec", cases=5 * 32, mini=32, clips="0.05,0.05,0.05")
+    a, b = run(_env=env, **kw), run(_env=env, between=75, **kw)
+    for i in range(3):
+        same_weights(a, b, str(i), str(i))
+        out, cost = b["out:%d" % i].astype(np.float64), b["cost:%d" % i]
+        assert (out[:, 0] > np.log(0.01)).all()
+        assert abs(-out[:, 0].sum() - cost[0]) <= 75 * 280 * U
+        assert (np.diff(out[:, 5:], axis=1) <= 0).all() and ((out[:, 1] >= 0) & (out[:, 1] <= np.log(10) + 1e-5)).all()
+    assert np.array_equal(a["norms"], b["norms"])
+
+
 def test_clip_norm_option(tmp_path):
     """--clip-norm on the command line, saved with the checkpoint and changed when resuming from it."""
     cfg = ["--layer-def=" + os.path.join(modelutil.CONFIGS, "layers-80sec.cfg"), "--layer-params=" + os.path.join(modelutil.CONFIGS, "layer-params-80sec.cfg")]
