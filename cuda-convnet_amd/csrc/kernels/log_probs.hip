@@ -13,7 +13,7 @@ namespace {
 constexpr int LT = 256;             // threads of a workgroup
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kMaxOut = 1 << 30;     // classes: their indices stay within an int wherever a tile ends
-constexpr float kHuge = 1e38f;      // from here on x * log2 e may overflow
+constexpr float kFar = 0x1p20f;     // a maximum so far from zero takes sums of its own: see far_from_zero
 
 struct LogProbArgs {
     const void* logits;
@@ -272,17 +272,16 @@ __device__ __forceinline__ float max_of(F x) {
     return r;
 }
 
-// t_j = (x_j - m) log2 e as fma(x_j, scale, -c), c = m log2 e as rounded; what the rounding of c moved every t by is known (another fma)
-// and taken back once for all.  Logits of kHuge and more are equal to m or so far below it that 2^t is 0; there any scale does that does
-// not overflow.  m = -inf leaves every t at -inf.
-struct Shift { float scale, c; };
-__device__ __forceinline__ Shift shift_for(float m) {
-    const bool huge = fabsf(m) >= kHuge && m != -INFINITY;
-    const float scale = huge ? 5.4210109e-20f : kLog2e;   // 2^-64
-    return {scale, fmaxf(m, huge ? m : -kHuge) * scale};
-}
+// t_j = (x_j - m) log2 e as fma(x_j, log2 e, -c), c = m log2 e as rounded; what the rounding of c moved every t by is known (another fma)
+// and taken back once for all.  It is half a step of c at most, 1/16 for |m| < 2^20; from there on it would cost w its accuracy, and from
+// 2^31 on 2^t its range, so that t is formed from x_j - m there (exact where 2^t counts), by far_sums(), and nothing is taken back.  (No half
+// is as large.)  m = -inf leaves every t at -inf.
+template <class T>
+__device__ __forceinline__ bool far_from_zero(float m) { return !__is_same(T, _Float16) && fabsf(m) >= kFar && m != -INFINITY; }
+struct Shift { float c; };
+__device__ __forceinline__ Shift shift_for(float m) { return {fmaxf(m, -1e30f) * kLog2e}; }
 __device__ __forceinline__ void take_back(float m, float& s, float& w) {
-    if (fabsf(m) >= kHuge) return;
+    if (!(fabsf(m) < kFar)) return;
     const float c = m * kLog2e, d = fmaf(m, kLog2e, -c), f = __builtin_amdgcn_exp2f(-d);
     w = (w - d * s) * f;
     s *= f;
@@ -298,7 +297,7 @@ __device__ __forceinline__ void sums_of(F t, float& s, float& w) {
         s += e;
         if (ENT) w = fmaf(e, x, w);
     }
-    asm volatile("" : "+v"(s));   // here, and not with every e kept until s is used
+    asm volatile("" : "+v"(s), "+v"(w));   // here, and not with every e kept until they are used
 }
 template <int COUNT, class F>
 __device__ __forceinline__ float guarded(F t) {
@@ -309,6 +308,20 @@ __device__ __forceinline__ float guarded(F t) {
         w = fmaf(__builtin_amdgcn_exp2f(x), fmaxf(x, -200.f), w);
     }
     return w;
+}
+// s and w of the logits x(0) ... x(COUNT - 1) for a maximum far from zero.
+template <bool ENT, int COUNT, class F>
+__device__ __forceinline__ void far_sums(F x, float m, float& s, float& w) {
+    float base = m;
+    s = w = 0.f;
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) {
+        if (i % 4 == 0) asm volatile("" : "+v"(base), "+v"(s));   // four at a time in registers, and nothing of before kept for here
+        const float t = (x(i) - base) * kLog2e, e = __builtin_amdgcn_exp2f(t);
+        s += e;
+        if (ENT) w = fmaf(e, fmaxf(t, -200.f), w);
+    }
+    asm volatile("" : "+v"(s));
 }
 
 // The largest element of a pack.
@@ -321,13 +334,13 @@ __device__ __forceinline__ float max_in(const Words<T, N>& v, Pass p) {
     for (int i = 1; i < v.COUNT; ++i) asm("v_pk_max_f16 %0, %1, %2" : "=v"(m.w[0]) : "v"(m.w[0]), "v"(v.w[i]));
     return fmaxf(m.at(0, p), m.at(1, p));
 }
-// Element k as fma(x, scale, -c); a half goes into the fma as it is (volatile: see Pass).
+// Element k as fma(x, log2 e, -c); a half goes into the fma as it is (volatile: see Pass).
 template <class T, int N>
 __device__ __forceinline__ float shifted(const Words<T, N>& v, int k, Shift h, Pass p) {
-    if (!__is_same(T, _Float16)) return fmaf(v.at(k, p), h.scale, -h.c);
+    if (!__is_same(T, _Float16)) return fmaf(v.at(k, p), kLog2e, -h.c);
     float t;
-    if (k % 2) asm volatile("v_fma_mix_f32 %0, %1, %2, -%3 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(t) : "v"(v.w[k / 2]), "v"(h.scale), "v"(h.c));
-    else asm volatile("v_fma_mix_f32 %0, %1, %2, -%3 op_sel:[0,0,0] op_sel_hi:[1,0,0]" : "=v"(t) : "v"(v.w[k / 2]), "v"(h.scale), "v"(h.c));
+    if (k % 2) asm volatile("v_fma_mix_f32 %0, %1, %2, -%3 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(t) : "v"(v.w[k / 2]), "v"(kLog2e), "v"(h.c));
+    else asm volatile("v_fma_mix_f32 %0, %1, %2, -%3 op_sel:[0,0,0] op_sel_hi:[1,0,0]" : "=v"(t) : "v"(v.w[k / 2]), "v"(kLog2e), "v"(h.c));
     return t;
 }
 
@@ -403,11 +416,14 @@ __global__ void __launch_bounds__(LT) __attribute__((amdgpu_waves_per_eu(4))) k_
         const Pass pass;
         sums_of<ENT, U * V>([&](int i) { return shifted(v[i / V], i % V, h, pass); }, s, w);
     }
-    if (ENT && __any(w != w)) {   // ruled-out classes (or NaN): again, with the guard that the usual case is spared
+    if (__any(far_from_zero<T>(m))) {
+        const Pass pass;
+        far_sums<ENT, U * V>([&](int i) { return v[i / V].at(i % V, pass); }, m, s, w);
+    } else if (ENT && __any(w != w)) {   // ruled-out classes (or NaN): again, with the guard that the usual case is spared
         Shift again = h;
         asm volatile("" : "+v"(again.c));   // (not the values of before, kept)
         const Pass pass;
-        w = guarded<U * V>([&](int i) { return fmaf(v[i / V].at(i % V, pass), again.scale, -again.c); });
+        w = guarded<U * V>([&](int i) { return fmaf(v[i / V].at(i % V, pass), kLog2e, -again.c); });
     }
     G::sum2(s, w, shRed[group] + G::WAVES);
     take_back(m, s, w);
@@ -538,11 +554,19 @@ __global__ void __launch_bounds__(LT) k_log_probs_cols(LogProbArgs a, Parts p, i
         m[k] = fmaxf(fmaxf(shM[0][g * P + k], shM[1][g * P + k]), fmaxf(shM[2][g * P + k], shM[3][g * P + k]));
         const Shift h = shift_for(m[k]);
         sums_of<ENT, U>([&](int i) { return shifted(v[i], k, h, second); }, s[k], w[k]);
-        if (ENT && __any(w[k] != w[k])) {   // (see the rows)
+        const bool far = far_from_zero<T>(m[k]);   // (see the rows; here lanes of several cases share a wave)
+        if (ENT && __any(!far && w[k] != w[k])) {
             Shift again = h;
             asm volatile("" : "+v"(again.c));
             const Pass pass;
-            w[k] = guarded<U>([&](int i) { return fmaf(v[i].at(k, pass), again.scale, -again.c); });
+            w[k] = guarded<U>([&](int i) { return fmaf(v[i].at(k, pass), kLog2e, -again.c); });
+        }
+        if (__any(far)) {
+            float fs, fw;
+            const Pass pass;
+            far_sums<ENT, U>([&](int i) { return v[i].at(k, pass); }, m[k], fs, fw);
+            s[k] = far ? fs : s[k];
+            w[k] = far ? fw : w[k];
         }
         s[k] = over_lanes(s[k], G, Sum());
         if (ENT) w[k] = over_lanes(w[k], G, Sum());
