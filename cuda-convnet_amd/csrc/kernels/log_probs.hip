@@ -256,8 +256,8 @@ __device__ __forceinline__ void write_top(const LogProbArgs& a, int n, int rank,
     a.topLogProbs[(size_t)rank * a.numCases + n] = key ? log_prob(key_logit(key), c) : -INFINITY;
 }
 
-// The largest of x(0) ... x(COUNT - 1), NaN left out, two a step.  (As asm: the compiler would first quieten every operand, one more
-// instruction each.)
+// The largest of x(0) ... x(COUNT - 1), quiet NaN left out, two a step.  (As asm: the compiler would first quieten every operand, one more
+// instruction each.  A signalling NaN hides what came before it; the sum tells that there may be one, and then number_max() is taken.)
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
     asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
@@ -270,6 +270,28 @@ __device__ __forceinline__ float max_of(F x) {
 #pragma unroll
     for (int i = 3; i < COUNT; i += 2) r = max3(r, x(i), x(i + 1 < COUNT ? i + 1 : i));
     return r;
+}
+
+// The largest number of x(0) ... x(COUNT - 1); -inf if there is none.
+template <int COUNT, class F>
+__device__ __forceinline__ float number_max(F x) {
+    float r = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) {
+        const float y = x(i);
+        r = y > r ? y : r;
+        asm volatile("" : "+v"(r));   // one after the other, in few registers
+    }
+    return r;
+}
+
+// Nothing that was formed of these elements before is kept for what follows.
+template <class T, int N, int U>
+__device__ __forceinline__ void hide(Words<T, N> (&v)[U]) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < Words<T, N>::COUNT; ++i) asm volatile("" : "+v"(v[u].w[i]));
 }
 
 // t_j = (x_j - m) log2 e as fma(x_j, log2 e, -c), c = m log2 e as rounded; what the rounding of c moved every t by is known (another fma)
@@ -404,12 +426,9 @@ __global__ void __launch_bounds__(LT) __attribute__((amdgpu_waves_per_eu(4))) k_
 #pragma unroll
         for (int u = 0; u < U; ++u) pm[u] = max_in(v[u], pass);
     }
-    const float mine = max_of<U>([&](int u) { return pm[u]; });
-    const float m = G::max(mine, shRed[group]);
-    if (TOP) {
-        shMax[threadIdx.x] = mine;
-        if (tid == 0) shCount[group] = shPacks[group] = 0;
-    }
+    float mine = max_of<U>([&](int u) { return pm[u]; });
+    float m = G::max(mine, shRed[group]);
+    if (TOP && tid == 0) shCount[group] = shPacks[group] = 0;
     float s, w;
     const Shift h = shift_for(m);
     {
@@ -427,6 +446,15 @@ __global__ void __launch_bounds__(LT) __attribute__((amdgpu_waves_per_eu(4))) k_
     }
     G::sum2(s, w, shRed[group] + G::WAVES);
     take_back(m, s, w);
+    if (s != s) {   // (in the whole group)
+        hide(v);
+        const Pass pass;
+#pragma unroll
+        for (int u = 0; u < U; ++u) pm[u] = number_max<V>([&](int k) { return v[u].at(k, pass); });
+        mine = number_max<U>([&](int u) { return pm[u]; });
+        m = G::max(mine, shRed[group]);
+    }
+    if (TOP) shMax[threadIdx.x] = mine;
     const CaseStats c = case_stats(m, s);
     if (tid == 0) {
         if (p.parts == 1) write_case(a, n, c, s, w, label, labelLogit);
@@ -493,7 +521,7 @@ __global__ void __launch_bounds__(LT) k_log_probs_cols(LogProbArgs a, Parts p, i
     constexpr int WINDOWS = U >= 2 ? 2 : 1, W = U / WINDOWS;   // the top's maxima are kept for W classes at a time
     constexpr int Q = P == 1 ? 8 : WINDOWS * P;
     extern __shared__ unsigned long long shDyn[];
-    __shared__ float shM[4][8 * P], shS[4][8 * P], shW[4][8 * P];
+    __shared__ float shM[4][8 * P], shS[4][8 * P], shW[4][8 * P], shLogSum[TOP ? 8 * P : 1], shMost[TOP ? 8 * P : 1];
     const int G = 1 << logG, R = LT >> logG, cases = G * P;
     const int g = threadIdx.x & (G - 1), r = threadIdx.x >> logG, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int tiles = (a.numCases + cases - 1) / cases;
@@ -576,17 +604,40 @@ __global__ void __launch_bounds__(LT) k_log_probs_cols(LogProbArgs a, Parts p, i
         }
     }
     __syncthreads();
+    const int cc = min(lane, cases - 1);   // (cases <= 64: every wave sees all of them)
+    float M = fmaxf(fmaxf(shM[0][cc], shM[1][cc]), fmaxf(shM[2][cc], shM[3][cc]));
+    float S = shS[0][cc] + shS[1][cc] + shS[2][cc] + shS[3][cc], Wt = shW[0][cc] + shW[1][cc] + shW[2][cc] + shW[3][cc];
+    take_back(M, S, Wt);
+    if (__any(S != S)) {   // (in the whole workgroup; see the rows)
+        __syncthreads();
+        hide(v);
+        const Pass pass;
+#pragma unroll
+        for (int k = 0; k < P; ++k) {
+            m[k] = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < WINDOWS; ++i) {
+                const float y = number_max<W>([&](int u) { return v[i * W + u].at(k, pass); });
+                if (TOP) {
+                    pm[i][k] = y;
+                    shSeg[(g * P + k) * (WINDOWS * R + 1) + i * R + r] = y;
+                }
+                m[k] = fmaxf(m[k], y);
+            }
+            m[k] = over_lanes(m[k], G, Larger());
+            if (lane < G) shM[wave][g * P + k] = m[k];
+        }
+        __syncthreads();
+        M = fmaxf(fmaxf(shM[0][cc], shM[1][cc]), fmaxf(shM[2][cc], shM[3][cc]));
+    }
     if ((int)threadIdx.x < cases) {
-        const int cc = threadIdx.x, n = myCase;
-        float M = fmaxf(fmaxf(shM[0][cc], shM[1][cc]), fmaxf(shM[2][cc], shM[3][cc]));
-        float S = shS[0][cc] + shS[1][cc] + shS[2][cc] + shS[3][cc], Wt = shW[0][cc] + shW[1][cc] + shW[2][cc] + shW[3][cc];
-        take_back(M, S, Wt);
+        const int n = myCase;
         if (p.parts == 1) {
             const CaseStats c = case_stats(M, S);
             write_case(a, n, c, S, Wt, label, labelLogit);
             if (TOP) {
-                shS[0][cc] = c.logSum;   // (these two are read by their own thread only until the next barrier)
-                shW[0][cc] = c.m;
+                shLogSum[cc] = c.logSum;
+                shMost[cc] = c.m;
             }
         } else p.stats[(size_t)n * p.parts + part] = {M, S, Wt, labelLogit};
     }
@@ -635,7 +686,7 @@ __global__ void __launch_bounds__(LT) k_log_probs_cols(LogProbArgs a, Parts p, i
     __syncthreads();
     const auto put = [&](int cc, int rank, unsigned long long key) {
         const int n = min((tile * G + cc / P) * P, a.numCases - P) + cc % P;
-        if (p.parts == 1) write_top(a, n, rank, key, CaseStats{shW[0][cc], shS[0][cc], 0.f});
+        if (p.parts == 1) write_top(a, n, rank, key, CaseStats{shMost[cc], shLogSum[cc], 0.f});
         else p.keys[((size_t)n * p.parts + part) * a.numTop + rank] = key;
     };
     const int count = owner < cases ? few ? len : shCount[owner] : 0;
