@@ -371,7 +371,10 @@ __device__ __forceinline__ float shifted(const Words<T, N>& v, int k, Shift h, P
 // rest there: the largest logit, the sums against it, the candidates for the top.  One pass over memory, and no rescaling of running
 // sums.  Long cases are bound by HBM with the vector units close behind (7 instructions an element, 80 ... 90 % busy): 2048 x 131072 bf16
 // (537 MB) with entropy and 20 alternatives 90 ... 100 us and 8 for joining, 5.0 ... 5.5 TB/s; reading alone takes 78.
-constexpr int kPacks = 128;
+// Packs that may hold candidates.  A threshold lets k + k / 4 + 1 of the lanes' maxima through at most (41 for k = 32; ties aside), and
+// with them, of s lanes of many packs each, s ln(s / (s - 41)) packs on average: 45 of a workgroup's, 65 of a wave's (81 the most of 4000 cases
+// of normal logits).  8192 x 1000 bf16 with 32 alternatives: 105 us with lists of 32 a wave, which nearly every case overflowed.
+constexpr int packs_for(int threads, int U) { return threads == LT ? 128 : U == 1 ? 64 : 112; }
 template <class T, int THREADS, int U, bool ENT, bool TOP, bool NT>
 __global__ void __launch_bounds__(LT) __attribute__((amdgpu_waves_per_eu(4))) k_log_probs_rows(LogProbArgs a, Parts p) {
     typedef Group<THREADS> G;
@@ -380,7 +383,8 @@ __global__ void __launch_bounds__(LT) __attribute__((amdgpu_waves_per_eu(4))) k_
     __shared__ float shMax[TOP ? LT : 1];
     __shared__ unsigned long long shCand[TOP ? GROUPS : 1][TOP ? kCand + MC_MAX_TOP : 1];
     // the packs that hold candidates, and where they are from
-    constexpr int PACKS = kPacks / GROUPS;
+    constexpr int PACKS = packs_for(THREADS, U);
+    static_assert(U == 1 || PACKS >= 2 * (MC_MAX_TOP + MC_MAX_TOP / 4 + 1), "");
     __shared__ unsigned shPack[TOP ? GROUPS : 1][TOP ? PACKS : 1][4], shFrom[TOP ? GROUPS : 1][TOP ? PACKS : 1];
     __shared__ int shPacks[GROUPS], shCount[GROUPS];
     const int group = G::index(), tid = G::tid();
