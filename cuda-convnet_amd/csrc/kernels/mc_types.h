@@ -121,12 +121,15 @@ inline bool with_type(int type, F f) {
 inline bool fits_a_grid(size_t blocks, int threads) { return blocks <= 0xffffffffu / (unsigned)threads; }
 
 // The stream a call names must belong to the current device: every pointer is taken to live there, and grids are sized for it.
+// Where the runtime cannot tell, the launch says; the error of asking is not left for launch_status to find (one that was there before is).
 inline bool stream_on_current_device(mcStream_t s) {
     if (!s) return true;
     int dev = 0;
     hipDevice_t of = 0;
-    if (hipGetDevice(&dev) != hipSuccess || hipStreamGetDevice(S(s), &of) != hipSuccess) return true;   // cannot tell: the launch says
-    return dev == (int)of;
+    const bool clean = hipPeekAtLastError() == hipSuccess;
+    if (hipGetDevice(&dev) == hipSuccess && hipStreamGetDevice(S(s), &of) == hipSuccess) return dev == (int)of;
+    if (clean) (void)hipGetLastError();
+    return true;
 }
 
 }  // namespace mc
