@@ -272,6 +272,8 @@ __device__ __forceinline__ float max_of(F x) {
     return r;
 }
 
+// Code for what hardly happens goes out of the way.
+__device__ __forceinline__ bool rare(bool v) { return __builtin_expect(v, 0); }
 // The largest number of x(0) ... x(COUNT - 1); -inf if there is none.
 template <int COUNT, class F>
 __device__ __forceinline__ float number_max(F x) {
@@ -432,14 +434,17 @@ __global__ void __launch_bounds__(LT) __attribute__((amdgpu_waves_per_eu(4))) k_
     }
     float mine = max_of<U>([&](int u) { return pm[u]; });
     float m = G::max(mine, shRed[group]);
-    if (TOP && tid == 0) shCount[group] = shPacks[group] = 0;
+    if (TOP) {
+        shMax[threadIdx.x] = mine;
+        if (tid == 0) shCount[group] = shPacks[group] = 0;
+    }
     float s, w;
     const Shift h = shift_for(m);
     {
         const Pass pass;
         sums_of<ENT, U * V>([&](int i) { return shifted(v[i / V], i % V, h, pass); }, s, w);
     }
-    if (__any(far_from_zero<T>(m))) {
+    if (rare(__any(far_from_zero<T>(m)))) {
         const Pass pass;
         far_sums<ENT, U * V>([&](int i) { return v[i / V].at(i % V, pass); }, m, s, w);
     } else if (ENT && __any(w != w)) {   // ruled-out classes (or NaN): again, with the guard that the usual case is spared
@@ -450,15 +455,15 @@ __global__ void __launch_bounds__(LT) __attribute__((amdgpu_waves_per_eu(4))) k_
     }
     G::sum2(s, w, shRed[group] + G::WAVES);
     take_back(m, s, w);
-    if (s != s) {   // (in the whole group)
+    if (rare(s != s)) {   // (in the whole group)
         hide(v);
         const Pass pass;
 #pragma unroll
         for (int u = 0; u < U; ++u) pm[u] = number_max<V>([&](int k) { return v[u].at(k, pass); });
         mine = number_max<U>([&](int u) { return pm[u]; });
         m = G::max(mine, shRed[group]);
+        if (TOP) shMax[threadIdx.x] = mine;
     }
-    if (TOP) shMax[threadIdx.x] = mine;
     const CaseStats c = case_stats(m, s);
     if (tid == 0) {
         if (p.parts == 1) write_case(a, n, c, s, w, label, labelLogit);
@@ -525,7 +530,8 @@ __global__ void __launch_bounds__(LT) k_log_probs_cols(LogProbArgs a, Parts p, i
     constexpr int WINDOWS = U >= 2 ? 2 : 1, W = U / WINDOWS;   // the top's maxima are kept for W classes at a time
     constexpr int Q = P == 1 ? 8 : WINDOWS * P;
     extern __shared__ unsigned long long shDyn[];
-    __shared__ float shM[4][8 * P], shS[4][8 * P], shW[4][8 * P], shLogSum[TOP ? 8 * P : 1], shMost[TOP ? 8 * P : 1];
+    __shared__ float shM[4][8 * P], shS[4][8 * P], shW[4][8 * P];
+    __shared__ int shNan;
     const int G = 1 << logG, R = LT >> logG, cases = G * P;
     const int g = threadIdx.x & (G - 1), r = threadIdx.x >> logG, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int tiles = (a.numCases + cases - 1) / cases;
@@ -574,6 +580,7 @@ __global__ void __launch_bounds__(LT) k_log_probs_cols(LogProbArgs a, Parts p, i
             for (int i = 0; i < WINDOWS; ++i) shSeg[(g * P + k) * (WINDOWS * R + 1) + i * R + r] = pm[i][k];
         if ((int)threadIdx.x < cases) shCount[threadIdx.x] = 0;
     }
+    if (threadIdx.x == 0) shNan = 0;
 #pragma unroll
     for (int k = 0; k < P; ++k) {
         m[k] = over_lanes(m[k], G, Larger());
@@ -581,39 +588,44 @@ __global__ void __launch_bounds__(LT) k_log_probs_cols(LogProbArgs a, Parts p, i
     }
     __syncthreads();
     const Pass second;
+    bool far = false;
 #pragma unroll
     for (int k = 0; k < P; ++k) {
         m[k] = fmaxf(fmaxf(shM[0][g * P + k], shM[1][g * P + k]), fmaxf(shM[2][g * P + k], shM[3][g * P + k]));
         const Shift h = shift_for(m[k]);
         sums_of<ENT, U>([&](int i) { return shifted(v[i], k, h, second); }, s[k], w[k]);
-        const bool far = far_from_zero<T>(m[k]);   // (see the rows; here lanes of several cases share a wave)
-        if (ENT && __any(!far && w[k] != w[k])) {
+        far |= far_from_zero<T>(m[k]);
+        if (ENT && __any(w[k] != w[k])) {   // (see the rows)
             Shift again = h;
             asm volatile("" : "+v"(again.c));
             const Pass pass;
             w[k] = guarded<U>([&](int i) { return fmaf(v[i].at(k, pass), kLog2e, -again.c); });
         }
-        if (__any(far)) {
+    }
+    if (rare(__any(far))) {   // (lanes of several cases share a wave)
+#pragma unroll
+        for (int k = 0; k < P; ++k) {
             float fs, fw;
             const Pass pass;
             far_sums<ENT, U>([&](int i) { return v[i].at(k, pass); }, m[k], fs, fw);
-            s[k] = far ? fs : s[k];
-            w[k] = far ? fw : w[k];
+            s[k] = far_from_zero<T>(m[k]) ? fs : s[k];
+            w[k] = far_from_zero<T>(m[k]) ? fw : w[k];
         }
+    }
+    bool nan = false;
+#pragma unroll
+    for (int k = 0; k < P; ++k) {
         s[k] = over_lanes(s[k], G, Sum());
+        nan |= s[k] != s[k];
         if (ENT) w[k] = over_lanes(w[k], G, Sum());
         if (lane < G) {
             shS[wave][g * P + k] = s[k];
             shW[wave][g * P + k] = w[k];
         }
     }
+    if (nan) shNan = 1;
     __syncthreads();
-    const int cc = min(lane, cases - 1);   // (cases <= 64: every wave sees all of them)
-    float M = fmaxf(fmaxf(shM[0][cc], shM[1][cc]), fmaxf(shM[2][cc], shM[3][cc]));
-    float S = shS[0][cc] + shS[1][cc] + shS[2][cc] + shS[3][cc], Wt = shW[0][cc] + shW[1][cc] + shW[2][cc] + shW[3][cc];
-    take_back(M, S, Wt);
-    if (__any(S != S)) {   // (in the whole workgroup; see the rows)
-        __syncthreads();
+    if (rare(shNan)) {   // (see the rows)
         hide(v);
         const Pass pass;
 #pragma unroll
@@ -632,16 +644,18 @@ __global__ void __launch_bounds__(LT) k_log_probs_cols(LogProbArgs a, Parts p, i
             if (lane < G) shM[wave][g * P + k] = m[k];
         }
         __syncthreads();
-        M = fmaxf(fmaxf(shM[0][cc], shM[1][cc]), fmaxf(shM[2][cc], shM[3][cc]));
     }
     if ((int)threadIdx.x < cases) {
-        const int n = myCase;
+        const int cc = threadIdx.x, n = myCase;
+        float M = fmaxf(fmaxf(shM[0][cc], shM[1][cc]), fmaxf(shM[2][cc], shM[3][cc]));
+        float S = shS[0][cc] + shS[1][cc] + shS[2][cc] + shS[3][cc], Wt = shW[0][cc] + shW[1][cc] + shW[2][cc] + shW[3][cc];
+        take_back(M, S, Wt);
         if (p.parts == 1) {
             const CaseStats c = case_stats(M, S);
             write_case(a, n, c, S, Wt, label, labelLogit);
             if (TOP) {
-                shLogSum[cc] = c.logSum;
-                shMost[cc] = c.m;
+                shS[0][cc] = c.logSum;   // (these two are read by their own thread only until the next barrier)
+                shW[0][cc] = c.m;
             }
         } else p.stats[(size_t)n * p.parts + part] = {M, S, Wt, labelLogit};
     }
@@ -690,7 +704,7 @@ __global__ void __launch_bounds__(LT) k_log_probs_cols(LogProbArgs a, Parts p, i
     __syncthreads();
     const auto put = [&](int cc, int rank, unsigned long long key) {
         const int n = min((tile * G + cc / P) * P, a.numCases - P) + cc % P;
-        if (p.parts == 1) write_top(a, n, rank, key, CaseStats{shMost[cc], shLogSum[cc], 0.f});
+        if (p.parts == 1) write_top(a, n, rank, key, CaseStats{shW[0][cc], shS[0][cc], 0.f});
         else p.keys[((size_t)n * p.parts + part) * a.numTop + rank] = key;
     };
     const int count = owner < cases ? few ? len : shCount[owner] : 0;
