@@ -1133,6 +1133,21 @@ void ConvNet::predict(Layer& logits, DevMat& labels, int numTop, float* out) {
         }
 }
 
+// Throws where one of the labels is no class of the layer, or of a cost layer that takes them from data matrix dataIdx: the pass indexes its
+// probabilities with them.
+void ConvNet::checkLabels(const HostMat& labels, int dataIdx, Layer& logits) {
+    std::vector<std::pair<Layer*, int>> classes(1, {&logits, logits.getNumOutputs()});
+    for (CostLayer* c : _costs) {
+        if (!dynamic_cast<LogregCostLayer*>(c) || c->getPrev().size() != 2) continue;
+        DataLayer* from = dynamic_cast<DataLayer*>(c->getPrev()[0]);
+        if (from && from->dataIdx() == dataIdx) classes.push_back({c, c->getPrev()[1]->getNumOutputs()});
+    }
+    for (const auto& of : classes)
+        for (size_t i = 0; i < labels.numel(); i++)
+            if (!(labels.data()[i] >= 0 && labels.data()[i] < of.second))
+                throw std::runtime_error(fmt("label %g of case %ld is no class of layer '%s'", labels.data()[i], (long)i, of.first->getName().c_str()));
+}
+
 void PredictWorker::releaseHost() {
     DataWorker::releaseHost();
     if (_out) {
@@ -1148,9 +1163,7 @@ void PredictWorker::run() {
     if (layer->getType() == "softmax") layer = layer->getPrev()[0];
     const HostMat& labels = *(*_data)[1];   // one row: either order of storage is the same
     if (labels.rows() != 1) throw std::runtime_error("predictions need one row of labels as the second data matrix");
-    for (size_t i = 0; i < labels.numel(); i++)   // (the cost layers of the pass index the probabilities with them)
-        if (!(labels.data()[i] >= 0 && labels.data()[i] < layer->getNumOutputs()))
-            throw std::runtime_error(fmt("label %g of case %ld is no class of layer '%s'", labels.data()[i], (long)i, layer->getName().c_str()));
+    _convNet->checkLabels(labels, 1, *layer);
     dp.setData(*_data);
     if (_out->fortran() || _out->rows() != dp.getNumCases() || _out->cols() != 2 + 2 * _numTop)
         throw std::runtime_error("prediction matrix must be C-ordered (numCases, 2 + 2 * numTop)");

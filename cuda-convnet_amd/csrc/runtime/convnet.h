@@ -149,6 +149,7 @@ public:
     void lastGradNorm(float* normAndFactor);   // synchronous: norm and factor of the last update under setGradClip
     // test-mode predictions of a layer's outputs (as logits): out, on the host, is (cases, 2 + 2 * numTop), see PredictWorker
     void predict(Layer& logits, DevMat& labels, int numTop, float* out);
+    void checkLabels(const HostMat& labels, int dataIdx, Layer& logits);   // of a prediction, before its pass
     void reset();
     void fprop(PASS_TYPE passType);
     void fprop(int miniIdx, PASS_TYPE passType);

@@ -151,7 +151,7 @@ static PyObject* startFeatureWriter(PyObject*, PyObject* args) {
 
 // startPredictions([data, labels, ..., out], layerIdx, numTop): test pass; row n of `out`, C-ordered (cases, 2 + 2 * numTop) float32,
 // receives for case n the log probability of its label, the entropy, the numTop likeliest classes and their log probabilities,
-// with layer layerIdx's outputs (a softmax layer's inputs) as the logits.  Every label is a class.  finishBatch collects it like any batch.
+// with layer layerIdx's outputs (a softmax layer's inputs) as the logits.  Every label is a class of that layer and of the net's cost.  finishBatch collects it like any batch.
 static PyObject* startPredictions(PyObject*, PyObject* args) {
     REQUIRE_MODEL();
     PyObject* data;
