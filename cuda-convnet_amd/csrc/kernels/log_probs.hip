@@ -371,8 +371,9 @@ __device__ __forceinline__ float shifted(const Words<T, N>& v, int k, Shift h, P
 // ---------------------------------------------------------------- a case's classes side by side
 // A workgroup (or wave) takes up to THREADS * U packs of 16 bytes of one case into registers in one burst of loads, and does all the
 // rest there: the largest logit, the sums against it, the candidates for the top.  One pass over memory, and no rescaling of running
-// sums.  Long cases are bound by HBM with the vector units close behind (7 instructions an element, 80 ... 90 % busy): 2048 x 131072 bf16
-// (537 MB) with entropy and 20 alternatives 90 ... 100 us and 8 for joining, 5.0 ... 5.5 TB/s; reading alone takes 78.
+// sums.  Long cases are bound by the vector units (7 instructions an element, 90 % busy) with HBM close behind: 2048 x 131072 bf16
+// (537 MB) with entropy and 20 alternatives 93.6 us back to back, joining included, 5.7 TB/s (traced one at a time 105 and 9); reading alone
+// takes 78.
 // Packs that may hold candidates.  A threshold lets k + k / 4 + 1 of the lanes' maxima through at most (41 for k = 32; ties aside), and
 // with them, of s lanes of many packs each, s ln(s / (s - 41)) packs on average: 45 of a workgroup's, 65 of a wave's (81 the most of 4000 cases
 // of normal logits).  8192 x 1000 bf16 with 32 alternatives: 105 us with lists of 32 a wave, which nearly every case overflowed.
@@ -514,9 +515,9 @@ __global__ void __launch_bounds__(LT) __attribute__((amdgpu_waves_per_eu(4))) k_
 
 // ---------------------------------------------------------------- a class's cases side by side
 // A workgroup takes 256 / G classes of G * P cases at a time, U times, into registers: lane (r, g) holds P neighbouring cases of class
-// r of each.  P states a lane are reduced over the lanes that share them, then over the waves.  Without alternatives HBM bounds it (32000 x
-// 2048 bf16, 131 MB, 34 us and 5 for joining); with them every workgroup looks for the best of each of its cases among few classes, which
-// takes the vector units longer than the loads: the same with 20 alternatives 94 and 12 (16 more for keeping the stretches' maxima, 7
+// r of each.  P states a lane are reduced over the lanes that share them, then over the waves.  Without alternatives the loads bound it (32000 x
+// 2048 bf16, 131 MB, traced 36.5 us and 5 for joining: lines in pieces of 128 bytes); with them every workgroup looks for the best of each of its
+// cases among few classes, which takes the vector units longer than the loads: the same with 20 alternatives 96 and 11 (16 more for keeping the stretches' maxima, 7
 // for thresholds, 31 for collecting what reaches them, 6 for ordering it).
 // LDS of the top alternatives: the candidate lists (or what top_by_scan needs), the stretches' maxima, the counts, the thresholds.  A list
 // holds what a threshold lets through with room to spare: of s stretches, k of whose maxima reach it, about s ln(s / (s - k)) classes do.
