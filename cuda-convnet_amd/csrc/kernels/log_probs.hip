@@ -517,8 +517,8 @@ __global__ void __launch_bounds__(LT) __attribute__((amdgpu_waves_per_eu(4))) k_
 // A workgroup takes 256 / G classes of G * P cases at a time, U times, into registers: lane (r, g) holds P neighbouring cases of class
 // r of each.  P states a lane are reduced over the lanes that share them, then over the waves.  Without alternatives the loads bound it (32000 x
 // 2048 bf16, 131 MB, traced 36.5 us and 5 for joining: lines in pieces of 128 bytes); with them every workgroup looks for the best of each of its
-// cases among few classes, which takes the vector units longer than the loads: the same with 20 alternatives 96 and 11 (16 more for keeping the stretches' maxima, 7
-// for thresholds, 31 for collecting what reaches them, 6 for ordering it).
+// cases among few classes, which takes the vector units longer than the loads: the same with 20 alternatives 96 and 11 (16 more for keeping the
+// stretches' maxima, 7 for thresholds, 31 for collecting what reaches them, 6 for ordering it).
 // LDS of the top alternatives: the candidate lists (or what top_by_scan needs), the stretches' maxima, the counts, the thresholds.  A list
 // holds what a threshold lets through with room to spare: of s stretches, k of whose maxima reach it, about s ln(s / (s - k)) classes do.
 __host__ __device__ constexpr int col_cand(int top) { return 2 * top + 32; }

@@ -489,7 +489,8 @@ int mc_compute_logreg_softmax_grad(const float* labels, const float* probs, floa
  *                                that are left hold class -1 and log probability -inf
  * Each output may be NULL (then it is not computed); topClasses and topLogProbs go together.  Sums are held in float32, whatever
  * `type` is.  Logits of -inf are classes that are ruled out; a case with nothing else has m = -inf, ln sum = 0, labelLogProbs = -inf
- * (0 for "no class"), entropy 0.  A case with a NaN or +inf logit gets NaN for its log sum, log probabilities and entropy.
+ * (0 for "no class"), entropy 0.  A case with a NaN or +inf logit gets NaN for its log sum, log probabilities and entropy; its maximum
+ * and best classes are those of its numbers (the maximum NaN where it has none above -inf).  Finite logits of any size give finite statistics.
  * workspace: mc_log_probs_workspace_bytes(...) bytes (0 = none), 16-byte aligned; calls that may overlap in time, captured ones
  * included, need one each.  Results do not depend on the run: no atomics decide an order.  Outputs must not overlap anything else.
  * The stream must belong to the current device, as must every pointer.  Matrices that would take 2^24 workgroups are refused (2^26 cases
